@@ -181,6 +181,122 @@ int iam_dense_status(iam_dense_t h);
 int iam_dense_unpack(const uint16_t* buckets_dev, int in_dim, int bucket_cols, uint16_t* w_out_dev,
                      void* stream);
 
+/* ------------------------------------------------------------------ operands of the operators below */
+enum { IAM_F32 = 0, IAM_F16 = 1, IAM_BF16 = 2 };
+/* Rows of heads on the device: element d of head j of row t is data[t * token_stride +
+ * j * head_stride + d] (strides in elements; the dims of a head are adjacent).  Rows may lie at
+ * any element offset and stride; 16-byte aligned ones are moved in 16-byte accesses. */
+typedef struct {
+    void* data;
+    long long token_stride, head_stride;
+} iam_rows;
+
+/* ------------------------------------------------------------------ rotary positions */
+/* rope_mx (aux.cl:227-248, with the table of attention.hpp:207-235) for any head: the first
+ * rot_dim dims turn in pairs, pair i of a token at position p by the angle p * w[i],
+ *     (a, b) -> f * (a cos - b sin, b cos + a sin),
+ * where pair i is dims (i, i + rot_dim/2), or (2i, 2i + 1) when `interleaved` is set.  The other
+ * dims are copied.  w[i] = theta^(-2i/rot_dim), changed by `scaling` for contexts `factor` times
+ * longer than the original_ctx tokens a model was trained on:
+ *   LINEAR  w / factor
+ *   NTK     theta * factor^(rot_dim / (rot_dim - 2)) in place of theta
+ *   BANDED  pairs that turn at least high_turns times (0: 4) in original_ctx tokens keep w, pairs
+ *           that turn at most low_turns times (0: 1) get w / factor, with a ramp in the turns between
+ *   YARN    the same with a ramp in the pair number between the pairs that turn high_turns
+ *           (0: 32) and low_turns (0: 1) times, and f = 0.1 ln(factor) + 1
+ * f is 1 otherwise; attn_factor > 0 sets it.  Angles are reduced in 64 bits, so they stay exact
+ * at any position; the rotation is in fp32 and rounded once. */
+enum { IAM_ROPE_NONE = 0, IAM_ROPE_LINEAR = 1, IAM_ROPE_NTK = 2, IAM_ROPE_YARN = 3, IAM_ROPE_BANDED = 4 };
+typedef struct {
+    int head_dim, rot_dim; /* rot_dim even, 2 .. head_dim <= 1024 */
+    int interleaved;       /* 0: half layout */
+    int scaling;           /* IAM_ROPE_* */
+    double theta;          /* above 1 */
+    double factor;         /* at least 1 (any scaling but NONE) */
+    int original_ctx;      /* YARN and BANDED */
+    double low_turns, high_turns, attn_factor; /* 0: the default */
+} iam_rope_config;
+typedef struct iam_rope_s* iam_rope_t;
+/* The rot_dim/2 frequencies w (radians per position) and the factor f (may be NULL) on the host;
+ * needs no GPU. */
+int iam_rope_frequencies(const iam_rope_config* cfg, double* radians_out, double* factor_out);
+/* A handle holds the frequencies on `device`; calls only read it, so any streams may share it. */
+int iam_rope_create(iam_rope_t* out, const iam_rope_config* cfg, int device);
+int iam_rope_destroy(iam_rope_t h);
+/* Rotates n_heads heads of q and n_kv_heads heads of k (0: none) of n_tokens tokens at
+ * positions_dev[t] (int32, any value) in one launch.  Output rows are the input rows themselves
+ * (the same pointer and strides) or do not overlap them. */
+int iam_rope_apply(iam_rope_t h, int dtype, int n_tokens, const int32_t* positions_dev, int n_heads, const iam_rows* q_in,
+                   const iam_rows* q_out, int n_kv_heads, const iam_rows* k_in, const iam_rows* k_out, void* stream);
+
+/* ------------------------------------------------------------------ 8-bit KV cache */
+/* A paged cache of keys and values in 8 bits with one fp32 scale per page and KV head, owned by
+ * the caller: codes [n_pages][n_kv_heads][page_size][head_dim], scales [n_pages][n_kv_heads], a
+ * value being code * scale.  Sequence i keeps token t in page block_table[i * max_pages + t /
+ * page_size], row t % page_size.  The scale of a page is the smallest power of two (at least
+ * 2^-126) that brings every value of the page and head within the largest code (127; 448 for
+ * e4m3): dividing by it is exact, so each value is rounded once (to nearest, ties to even), and a
+ * page whose scale grows when larger values are appended shifts its older codes. */
+enum { IAM_KV8_INT8 = 0, IAM_KV8_E4M3 = 1 };
+typedef struct {
+    int format;           /* IAM_KV8_* */
+    int n_pages, page_size; /* page_size 16, 32, 64 or 128 */
+    int n_kv_heads, head_dim; /* head_dim 64, 128 or 256 */
+    void *k, *v;          /* codes, 16-byte aligned */
+    float *k_scale, *v_scale;
+    const int32_t* block_table;
+    int n_seqs, max_pages;
+} iam_kv8_cache;
+typedef struct iam_kv8_s* iam_kv8_t;
+/* A handle owns the scratch of the attention's split context (about 20 to 80 MB, set by head_dim;
+ * never reallocated, so captured graphs keep it) and an error word.  One handle per stream: calls
+ * of one handle must not overlap on the GPU, graphs captured with it included. */
+int iam_kv8_create(iam_kv8_t* out, int n_heads, int n_kv_heads, int head_dim, int device);
+int iam_kv8_destroy(iam_kv8_t h);
+/* Both calls take ragged rows: sequence i owns rows [cu_dev[i], cu_dev[i + 1]) (int32, n_seqs + 1
+ * values, cu_dev[0] = 0; NULL: one row per sequence), the LAST tokens of the seq_lens_dev[i]
+ * tokens that it has with them; n_rows is the row capacity of the buffers.  Rows behind the last
+ * sequence are neither read nor written.
+ *
+ * iam_kv8_append: rounds the new tokens' keys and values into their pages.  A page being
+ * written belongs to one sequence and appears once in its table; rows of a page behind the
+ * sequence's last token keep their bytes.  Infinities become the largest code, NaN becomes 0, and neither enters
+ * the scale. */
+int iam_kv8_append(iam_kv8_t h, const iam_kv8_cache* cache, int dtype, int n_rows, const iam_rows* k, const iam_rows* v,
+                   const int32_t* cu_dev, const int32_t* seq_lens_dev, void* stream);
+/* Causal attention of the rows over their sequences: the row at position p sees tokens
+ * (p - window, p] (window 0: all up to p); query head j reads KV head j / (n_heads / n_kv_heads).
+ * scale 0: 1/sqrt(head_dim).  out has q's dtype; lse_dev (may be NULL) [n_rows][n_heads] fp32
+ * receives the natural logarithm of the sum of exponentials.  A row that sees nothing (a position
+ * below 0) gives 0 and -inf.  max_q: a bound on one sequence's rows, if known (0: n_rows); it
+ * chooses the kernel and never the result's meaning.  What stands in a page behind the sequence's
+ * last token has no influence. */
+int iam_kv8_attention(iam_kv8_t h, const iam_kv8_cache* cache, int dtype, int n_rows, int max_q, const iam_rows* q,
+                      const int32_t* cu_dev, const int32_t* seq_lens_dev, float scale, int window, const iam_rows* out,
+                      float* lse_dev, void* stream);
+/* Synchronises the device; IAM_ERR_ARG when a call of `h` since the last iam_kv8_status met a page
+ * number outside the cache, a sequence longer than its table, a negative length or row offsets
+ * that do not ascend within n_rows (such tokens or sequences are skipped); the word is then cleared.
+ * Tokens before position 0 (more rows than the sequence has tokens, as in the padding of a batch) are
+ * skipped without an error. */
+int iam_kv8_status(iam_kv8_t h);
+
+/* ------------------------------------------------------------------ log probabilities */
+/* For each row of logits_dev [n_rows][row_stride] (vocab of them used): logprob = the log
+ * softmax at targets_dev[row], lse = log of the sum of exponentials, entropy (nats), rank = the
+ * number of tokens ahead of the target (larger logit, or equal and of a lower index), and the
+ * top_k (0 .. 64, at most vocab) largest log probabilities with their tokens, ties to the lower
+ * index, in top_logprob_dev / top_index_dev [n_rows][top_k].  Any output but those of a positive
+ * top_k may be NULL.  A negative target is none: logprob 0, rank -1; a target of vocab or more
+ * gives NaN and -1.  Logits of -inf are tokens with no probability; a row of nothing else, or with a
+ * NaN or +inf, has no distribution: its logprob, entropy and top log probabilities are NaN (lse:
+ * -inf for the former, NaN for the latter; with a NaN the top tokens are not specified).  Rows start
+ * at any element; row_stride * element size is below 1 MiB of logits per row (IAM_ERR_UNSUPPORTED
+ * above).  Runs on the current device. */
+int iam_logprobs(const void* logits_dev, int dtype, int n_rows, int vocab, long long row_stride, const int32_t* targets_dev,
+                 float* logprob_dev, float* lse_dev, float* entropy_dev, int32_t* rank_dev, int top_k, float* top_logprob_dev,
+                 int32_t* top_index_dev, void* stream);
+
 /* ------------------------------------------------------------------ decode model */
 /* Replaces MistralModel (model.hpp:84-237), TransformerLayer (transformer_layer.hpp:55-162),
  * Attention (attention.hpp:71-404) and FeedForward (feedforward.hpp:89-183).  The model

@@ -226,6 +226,289 @@ class Dense:
         check(self.lib.iam_dense_status(self.h))
 
 
+# ---------------------------------------------------------------- rotary positions, 8-bit KV cache, log probabilities
+
+class _Rows(ctypes.Structure):
+    """iam_rows (include/iam_b200.h)."""
+    _fields_ = [("data", _vp), ("token_stride", _i64), ("head_stride", _i64)]
+
+
+class _RopeConfig(ctypes.Structure):
+    """iam_rope_config."""
+    _fields_ = [("head_dim", _i32), ("rot_dim", _i32), ("interleaved", _i32), ("scaling", _i32),
+                ("theta", ctypes.c_double), ("factor", ctypes.c_double), ("original_ctx", _i32),
+                ("low_turns", ctypes.c_double), ("high_turns", ctypes.c_double), ("attn_factor", ctypes.c_double)]
+
+
+class _KV8Cache(ctypes.Structure):
+    """iam_kv8_cache."""
+    _fields_ = [("format", _i32), ("n_pages", _i32), ("page_size", _i32), ("n_kv_heads", _i32), ("head_dim", _i32),
+                ("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("block_table", _vp), ("n_seqs", _i32),
+                ("max_pages", _i32)]
+
+
+_SIGNATURES.update({
+    "iam_rope_frequencies": [_vp, _vp, _vp],
+    "iam_rope_create": [_vp, _vp, _i32],
+    "iam_rope_destroy": [_vp],
+    "iam_rope_apply": [_vp, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _vp],
+    "iam_kv8_create": [_vp, _i32, _i32, _i32, _i32],
+    "iam_kv8_destroy": [_vp],
+    "iam_kv8_append": [_vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp],
+    "iam_kv8_attention": [_vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _f32, _i32, _vp, _vp, _vp],
+    "iam_kv8_status": [_vp],
+    "iam_logprobs": [_vp, _i32, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp],
+})
+
+ROPE_SCALINGS = ("none", "linear", "ntk", "yarn", "banded")
+KV8_INT8, KV8_E4M3 = 0, 1
+
+
+def _refuse(why):
+    raise IamError(IAM_ERR_ARG, why)
+
+
+def _dtype_code(t, what):
+    import torch
+    codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    code = codes.get(t.dtype)
+    if code is None:
+        _refuse(f"{what}: dtype must be float32, float16 or bfloat16, not {t.dtype}")
+    return code
+
+
+def _on(t, device, what, dtype=None, shape=None, contiguous=True):
+    """Checks one tensor argument: on CUDA device `device`, of `dtype` and `shape` where given."""
+    if not t.is_cuda or t.device.index != device:
+        _refuse(f"{what}: expected a tensor on cuda:{device}, not {t.device}")
+    if dtype is not None and t.dtype != dtype:
+        _refuse(f"{what}: expected {dtype}, not {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        _refuse(f"{what}: expected shape {tuple(shape)}, not {tuple(t.shape)}")
+    if contiguous and not t.is_contiguous():
+        _refuse(f"{what}: expected a contiguous tensor")
+    return t
+
+
+def _rows(t, device, what, dtype, n_rows, n_heads, head_dim):
+    """iam_rows of a [rows][heads][head_dim] tensor whose dims of a head are adjacent."""
+    _on(t, device, what, dtype, (n_rows, n_heads, head_dim), contiguous=False)
+    if t.stride(2) != 1:
+        _refuse(f"{what}: the dims of a head must be adjacent")
+    return _Rows(t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _stream_of(device, stream):
+    import torch
+    return (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
+
+
+def _no_overlap(out, what):
+    """An output whose rows share memory (an expanded tensor) would be written by several threads at once."""
+    if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
+        _refuse(f"{what}: an output's rows must not share memory")
+
+
+class Rope:
+    """Rotary positions (iam_rope_*): the first rot_dim dims of each head turn in pairs, half layout
+    (i, i + rot_dim/2) or interleaved (2i, 2i + 1), with frequencies theta^(-2i/rot_dim) scaled for contexts
+    `factor` times longer than original_ctx ("linear", "ntk", "yarn", "banded"; include/iam_b200.h)."""
+
+    def __init__(self, head_dim, rot_dim=None, interleaved=False, theta=1e6, scaling="none", factor=1.0, original_ctx=0,
+                 low_turns=0.0, high_turns=0.0, attn_factor=0.0, device=0):
+        self.lib, self.h, self.device, self.head_dim = load_library(), ctypes.c_void_p(), device, head_dim
+        self.cfg = self.config(head_dim, rot_dim, interleaved, theta, scaling, factor, original_ctx, low_turns, high_turns,
+                               attn_factor)
+        check(self.lib.iam_rope_create(ctypes.byref(self.h), ctypes.byref(self.cfg), device))
+
+    @staticmethod
+    def config(head_dim, rot_dim=None, interleaved=False, theta=1e6, scaling="none", factor=1.0, original_ctx=0,
+               low_turns=0.0, high_turns=0.0, attn_factor=0.0):
+        if scaling not in ROPE_SCALINGS:
+            _refuse(f"rope: scaling must be one of {', '.join(ROPE_SCALINGS)}")
+        return _RopeConfig(head_dim, head_dim if rot_dim is None else rot_dim, int(bool(interleaved)),
+                           ROPE_SCALINGS.index(scaling), theta, factor, original_ctx, low_turns, high_turns, attn_factor)
+
+    @staticmethod
+    def frequencies(cfg):
+        """-> (radians per position of each pair, factor on the rotated values) of a config(); needs no GPU."""
+        w, f = (ctypes.c_double * max(1, cfg.rot_dim // 2))(), ctypes.c_double()
+        check(load_library().iam_rope_frequencies(ctypes.byref(cfg), w, ctypes.byref(f)))
+        return list(w), f.value
+
+    def close(self):
+        if self.h:
+            self.lib.iam_rope_destroy(self.h)
+            self.h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def apply(self, q, positions, out=None, k=None, k_out=None, stream=None):
+        """Rotates q [tokens][heads][head_dim] (and k) at int32 `positions` [tokens] into out / k_out
+        (None: in place).  Rows may be strided; outputs are their inputs or do not overlap them."""
+        import torch
+        n = q.shape[0]
+        code = _dtype_code(q, "rope q")
+        out = q if out is None else out
+        qi = _rows(q, self.device, "rope q", None, n, q.shape[1], self.head_dim)
+        qo = _rows(out, self.device, "rope out", q.dtype, n, q.shape[1], self.head_dim)
+        _no_overlap(out, "rope out")
+        ki = ko = None
+        kh = 0
+        if k is not None:
+            kh = k.shape[1]
+            k_out = k if k_out is None else k_out
+            ki = _rows(k, self.device, "rope k", q.dtype, n, kh, self.head_dim)
+            ko = _rows(k_out, self.device, "rope k_out", q.dtype, n, kh, self.head_dim)
+            _no_overlap(k_out, "rope k_out")
+        _on(positions, self.device, "rope positions", torch.int32, (n,))
+        check(self.lib.iam_rope_apply(self.h, code, n, positions.data_ptr(), q.shape[1], ctypes.byref(qi), ctypes.byref(qo),
+                                      kh, None if ki is None else ctypes.byref(ki), None if ko is None else ctypes.byref(ko),
+                                      _stream_of(self.device, stream)))
+
+
+class KV8Cache:
+    """A paged 8-bit KV cache (iam_kv8_cache) over the caller's tensors: k / v codes
+    [n_pages][n_kv_heads][page_size][head_dim] (int8 or float8_e4m3fn), fp32 scales [n_pages][n_kv_heads], int32
+    block_table [n_seqs][max_pages].  Keeps the tensors alive."""
+
+    def __init__(self, k, v, k_scale, v_scale, block_table):
+        import torch
+        formats = {torch.int8: KV8_INT8, torch.float8_e4m3fn: KV8_E4M3}
+        if k.dtype not in formats or k.dim() != 4:
+            _refuse("kv8 cache: codes must be int8 or float8_e4m3fn [n_pages][n_kv_heads][page_size][head_dim]")
+        dev = k.device.index
+        _on(k, dev, "kv8 k")
+        _on(v, dev, "kv8 v", k.dtype, k.shape)
+        _on(k_scale, dev, "kv8 k_scale", torch.float32, k.shape[:2])
+        _on(v_scale, dev, "kv8 v_scale", torch.float32, k.shape[:2])
+        _on(block_table, dev, "kv8 block_table", torch.int32)
+        if block_table.dim() != 2:
+            _refuse("kv8 block_table: expected [n_seqs][max_pages]")
+        self.tensors = (k, v, k_scale, v_scale, block_table)
+        self.device, self.n_seqs, self.n_kv_heads, self.head_dim = dev, block_table.shape[0], k.shape[1], k.shape[3]
+        self.c = _KV8Cache(formats[k.dtype], k.shape[0], k.shape[2], k.shape[1], k.shape[3], k.data_ptr(), v.data_ptr(),
+                           k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), block_table.shape[0],
+                           block_table.shape[1])
+
+    @classmethod
+    def empty(cls, n_pages, n_kv_heads, page_size, head_dim, block_table, fmt="e4m3"):
+        """A cache of new tensors on the block table's device ("int8" or "e4m3" codes)."""
+        import torch
+        if fmt not in ("int8", "e4m3"):
+            _refuse("kv8 cache: format must be int8 or e4m3")
+        dt = torch.int8 if fmt == "int8" else torch.float8_e4m3fn
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        new = [torch.zeros(shape, dtype=torch.uint8, device=block_table.device).view(dt) for _ in range(2)]
+        scales = [torch.full(shape[:2], 2.0 ** -126, device=block_table.device) for _ in range(2)]
+        return cls(*new, *scales, block_table)
+
+
+class KV8:
+    """Append to and attention over 8-bit paged caches (iam_kv8_*).  One handle per stream: it owns the scratch
+    of contexts that several CTAs share, never reallocated."""
+
+    def __init__(self, n_heads, n_kv_heads, head_dim, device=0):
+        self.lib, self.h = load_library(), ctypes.c_void_p()
+        self.n_heads, self.n_kv_heads, self.head_dim, self.device = n_heads, n_kv_heads, head_dim, device
+        check(self.lib.iam_kv8_create(ctypes.byref(self.h), n_heads, n_kv_heads, head_dim, device))
+
+    def close(self):
+        if self.h:
+            self.lib.iam_kv8_destroy(self.h)
+            self.h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def status(self):
+        """Synchronises; raises IamError(IAM_ERR_ARG) if a call since the last status met a page, length or row
+        offset out of range."""
+        check(self.lib.iam_kv8_status(self.h))
+
+    def _common(self, cache, seq_lens, cu, what):
+        import torch
+        if cache.device != self.device:
+            _refuse(f"{what}: the cache is on another device than the handle")
+        _on(seq_lens, self.device, what + " seq_lens", torch.int32, (cache.n_seqs,))
+        if cu is not None:
+            _on(cu, self.device, what + " cu", torch.int32, (cache.n_seqs + 1,))
+
+    def append(self, cache, k, v, seq_lens, cu=None, stream=None):
+        """Rounds k, v [rows][n_kv_heads][head_dim] into their pages; sequence i owns rows cu[i] .. cu[i + 1]
+        (None: row i) and they are the last of its seq_lens[i] tokens."""
+        self._common(cache, seq_lens, cu, "kv8 append")
+        n = k.shape[0]
+        code = _dtype_code(k, "kv8 append k")
+        kr = _rows(k, self.device, "kv8 append k", None, n, self.n_kv_heads, self.head_dim)
+        vr = _rows(v, self.device, "kv8 append v", k.dtype, n, self.n_kv_heads, self.head_dim)
+        check(self.lib.iam_kv8_append(self.h, ctypes.byref(cache.c), code, n, ctypes.byref(kr), ctypes.byref(vr),
+                                      None if cu is None else cu.data_ptr(), seq_lens.data_ptr(),
+                                      _stream_of(self.device, stream)))
+
+    def attention(self, cache, q, seq_lens, out, cu=None, max_q=0, scale=0.0, window=0, lse=None, stream=None):
+        """Causal attention of q [rows][n_heads][head_dim] over the sequences' tokens into `out` (q's dtype);
+        lse (fp32 [rows][n_heads]) receives the log of the sums.  max_q: a bound on one sequence's rows."""
+        import torch
+        self._common(cache, seq_lens, cu, "kv8 attention")
+        n = q.shape[0]
+        code = _dtype_code(q, "kv8 attention q")
+        qr = _rows(q, self.device, "kv8 attention q", None, n, self.n_heads, self.head_dim)
+        ro = _rows(out, self.device, "kv8 attention out", q.dtype, n, self.n_heads, self.head_dim)
+        _no_overlap(out, "kv8 attention out")
+        if lse is not None:
+            _on(lse, self.device, "kv8 attention lse", torch.float32, (n, self.n_heads))
+        check(self.lib.iam_kv8_attention(self.h, ctypes.byref(cache.c), code, n, max_q, ctypes.byref(qr),
+                                         None if cu is None else cu.data_ptr(), seq_lens.data_ptr(), scale, window,
+                                         ctypes.byref(ro), None if lse is None else lse.data_ptr(),
+                                         _stream_of(self.device, stream)))
+
+
+def logprobs(logits, targets=None, logprob=None, lse=None, entropy=None, rank=None, top_logprob=None, top_index=None,
+             stream=None):
+    """iam_logprobs over rows of logits [rows][vocab] (rows may be strided): log probability and rank of int32
+    `targets`, log of the sum of exponentials, entropy, and the best alternatives into top_logprob / top_index
+    [rows][top_k].  Any output may be None."""
+    import torch
+    if logits.dim() != 2 or not logits.is_cuda or logits.stride(1) != 1:
+        _refuse("logprobs: logits must be [rows][vocab] on a CUDA device, the tokens of a row adjacent")
+    n, vocab = logits.shape
+    dev = logits.device.index
+    code = _dtype_code(logits, "logprobs")
+    if targets is not None:
+        _on(targets, dev, "logprobs targets", torch.int32, (n,))
+    for t, what, dt in ((logprob, "logprob", torch.float32), (lse, "lse", torch.float32), (entropy, "entropy", torch.float32),
+                        (rank, "rank", torch.int32)):
+        if t is not None:
+            _on(t, dev, "logprobs " + what, dt, (n,))
+    if (top_logprob is None) != (top_index is None):
+        _refuse("logprobs: top_logprob and top_index come together")
+    k = 0
+    if top_logprob is not None:
+        k = top_logprob.shape[-1]
+        _on(top_logprob, dev, "logprobs top_logprob", torch.float32, (n, k))
+        _on(top_index, dev, "logprobs top_index", torch.int32, (n, k))
+    args = (logits.data_ptr(), code, n, vocab, logits.stride(0), _opt(targets), _opt(logprob), _opt(lse), _opt(entropy),
+            _opt(rank), k, _opt(top_logprob), _opt(top_index), _stream_of(dev, stream))
+    lib = load_library()
+    if dev == torch.cuda.current_device():
+        check(lib.iam_logprobs(*args))
+    else:
+        with torch.cuda.device(dev):
+            check(lib.iam_logprobs(*args))
+
+
+def _opt(t):
+    return None if t is None else t.data_ptr()
+
+
 # ---------------------------------------------------------------- decode model
 
 class ModelConfig(ctypes.Structure):
