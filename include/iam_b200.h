@@ -291,8 +291,7 @@ int iam_kv8_status(iam_kv8_t h);
  * gives NaN and -1.  Logits of -inf are tokens with no probability; a row of nothing else, or with a
  * NaN or +inf, has no distribution: its logprob, entropy and top log probabilities are NaN (lse:
  * -inf for the former, NaN for the latter; with a NaN the top tokens are not specified).  Rows start
- * at any element; row_stride * element size is below 1 MiB of logits per row (IAM_ERR_UNSUPPORTED
- * above).  Runs on the current device. */
+ * at any element.  Runs on the current device. */
 int iam_logprobs(const void* logits_dev, int dtype, int n_rows, int vocab, long long row_stride, const int32_t* targets_dev,
                  float* logprob_dev, float* lse_dev, float* entropy_dev, int32_t* rank_dev, int top_k, float* top_logprob_dev,
                  int32_t* top_index_dev, void* stream);

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(AppendParams
     if (lo >= hi) return;
     const int id = p.c.block_table[(size_t)seq * p.c.max_pages + index];
     if (id < 0 || id >= p.c.n_pages) {
-        if (tid == 0) *p.err = 1u;
+        if (tid == 0) atomicOr(p.err, kKv8ErrRange);
         return;
     }
     const size_t slot = (size_t)id * p.c.n_kv_heads + head;
@@ -181,6 +181,7 @@ int check_cache(const iam_kv8_cache* c) {
         return fail(IAM_ERR_UNSUPPORTED, "kv8: head_dim must be 64, 128 or 256");
     if (c->n_kv_heads <= 0 || c->n_pages <= 0 || c->max_pages <= 0 || c->n_seqs < 0) return fail(IAM_ERR_ARG, "kv8: bad cache sizes");
     if (c->n_kv_heads > 65535) return fail(IAM_ERR_ARG, "kv8: more than 65535 KV heads");
+    if ((long long)c->n_pages * c->n_kv_heads * c->page_size > INT32_MAX) return fail(IAM_ERR_UNSUPPORTED, "kv8: more than 2^31 rows of codes");
     if (!c->k || !c->v || !c->k_scale || !c->v_scale || (c->n_seqs > 0 && !c->block_table)) return fail(IAM_ERR_ARG, "kv8: null cache array");
     if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16)
         return fail(IAM_ERR_ARG, "kv8: codes must be 16-byte aligned");
@@ -220,7 +221,7 @@ extern "C" int iam_kv8_create(iam_kv8_t* out, int n_heads, int n_kv_heads, int h
     h->n_kv_heads = n_kv_heads;
     h->head_dim = head_dim;
     h->s.max_ctas = kv8_max_ctas(sms);
-    h->s.part_floats = kv8_part_floats(head_dim, sms);
+    h->s.part_floats = std::max(kv8_decode_part_floats(head_dim, sms), kv8_rows_part_floats(head_dim, sms));
     cudaError_t e = cudaMalloc(&h->s.part, h->s.part_floats * sizeof(float));
     if (e == cudaSuccess) e = cudaMalloc(&h->s.ctr, h->s.max_ctas * sizeof(int));
     if (e == cudaSuccess) e = cudaMemset(h->s.ctr, 0, h->s.max_ctas * sizeof(int));
@@ -256,6 +257,7 @@ extern "C" int iam_kv8_status(iam_kv8_t h) {
     IAM_CUDA_TRY(cudaMemcpy(&e, h->s.err, sizeof(e), cudaMemcpyDeviceToHost));
     if (!e) return IAM_OK;
     IAM_CUDA_TRY(cudaMemset(h->s.err, 0, sizeof(e)));
+    if (e & kKv8ErrWait) return fail(IAM_ERR_TIMEOUT, "kv8: a wait of the attention gave up");
     return fail(IAM_ERR_ARG, "kv8: a page number, a length or a row offset was out of range");
 }
 

@@ -49,7 +49,7 @@ IAM_DEV SeqRows seq_rows(const iam_kv8_cache& c, const int32_t* cu, const int32_
     r.len = ok ? r.len : 0;
     const long long room = (long long)c.max_pages * c.page_size;
     r.cap = r.len <= room ? r.len : (int)room;
-    if ((!ok || r.len > room) && err) *err = 1u;
+    if ((!ok || r.len > room) && err) atomicOr(err, kKv8ErrRange);
     r.start = r.len - r.n;
     return r;
 }

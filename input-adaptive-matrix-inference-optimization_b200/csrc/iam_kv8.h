@@ -11,6 +11,8 @@ namespace iam {
 
 constexpr int kKv8MaxItems = 1 << 16;  // row tiles of one attention call at most
 constexpr int kKv8Group = 16;          // tokens that share a page for sure (the smallest page)
+constexpr unsigned kKv8ErrRange = 1u;  // error word: a page, length or row offset out of range
+constexpr unsigned kKv8ErrWait = 2u;   // a bounded wait gave up
 
 // Scratch of a handle: partial results of row tiles whose context is split over several CTAs, the
 // arrival counters of their joins (zero between calls) and the row-tile kernel's schedule.
@@ -37,7 +39,8 @@ struct Kv8Attn {
 
 int kv8_decode_launch(const Kv8Attn& a, int dtype, cudaStream_t s);
 int kv8_rows_launch(const Kv8Attn& a, int dtype, cudaStream_t s);
-size_t kv8_part_floats(int head_dim, int sms);
+size_t kv8_decode_part_floats(int head_dim, int sms);
+size_t kv8_rows_part_floats(int head_dim, int sms);
 int kv8_max_ctas(int sms);
 size_t kv8_plan_words();
 

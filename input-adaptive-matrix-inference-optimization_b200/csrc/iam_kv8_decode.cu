@@ -3,28 +3,40 @@
 // out = sum_t softmax_t(scale q.k_t) v_t in one pass with a running maximum and sum.  The rows of a
 // (sequence, KV head), up to 8, are the N of the tensor cores' m16n8k16 and the tokens (for the scores)
 // or the dims (for the values) its M, so a code enters one MMA and no row of the tile is padding for
-// want of queries.  The codes go from global memory into the registers of the fragments they belong to:
-// which physical dim plays a fragment's k (scores) or row (values) is free as long as the queries and
-// the output agree, and the choice below makes every access 16 bytes of adjacent codes of one token.
+// want of queries.  Which physical dim plays a fragment's k (scores) or row (values) is free as long as the
+// queries and the output agree: the choice below makes every access 16 bytes of adjacent codes of one token.
+#include <climits>
 #include <algorithm>
 #include <atomic>
 
 #include "iam_kv8.cuh"
+#include "iam_tc.cuh"
 
 namespace iam {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
-constexpr int kTile = kWarps * kKv8Group;  // tokens of a work unit: one group for each warp
-constexpr int kMinUnits = 2;               // work units of a CTA at least, while there are enough
+constexpr int kMinUnits = 8;  // work units of a CTA at least, while there are enough
 
-// The call's work: units of kTile tokens, in the order (sequence, KV head, row tile, token), cut into
-// equal runs, one per CTA, whatever the sequences' lengths.
+// Warps of a CTA (one CTA an SM) and groups of 16 tokens in each warp's ring: 192 KB of codes on their way.
+template <int HD>
+struct Shape {
+    static constexpr int kWarps = HD == 256 ? 8 : 16;
+    static constexpr int kThreads = 32 * kWarps;
+    static constexpr int kHalves = HD == 256 ? 2 : 1;          // 128-byte columns of a row
+    static constexpr int kBox = kKv8Group * HD / kHalves;      // bytes of one copy
+    static constexpr int kStage = 2 * kHalves * kBox;          // a group's keys and values
+    static constexpr int kStages = 192 * 1024 / (kWarps * kStage);
+    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kPitch = HD + 4;
+    static_assert(kWarps * 8 * kPitch * 4 <= kRing, "the warps' results are joined where the codes were");
+};
+
+// The call's work: groups of 16 tokens in the order (sequence, KV head, row tile, token), cut into equal runs, one
+// per CTA, whatever the sequences' lengths.
 struct Item {
-    int rt, nt;      // row tiles of the sequence, units of one
-    int lo;          // first token read (a multiple of kKv8Group)
-    long long units; // of the whole sequence
+    int rt, nt;    // row tiles of the sequence, groups of one
+    int lo;        // first token read (a multiple of kKv8Group)
+    int units;     // of the whole sequence (the sum over the sequences is checked against 2^31)
 };
 
 template <int RT>
@@ -32,10 +44,21 @@ IAM_DEV Item item_of(const Kv8Attn& p, const SeqRows& r) {
     Item it;
     it.rt = (r.n * p.gq + RT - 1) / RT;
     it.lo = p.window > 0 ? max(0, r.start - p.window + 1) & ~(kKv8Group - 1) : 0;
-    it.nt = max(1, (r.cap - it.lo + kTile - 1) / kTile);  // a sequence without tokens still gets its rows written
-    it.units = (long long)it.rt * it.nt * p.c.n_kv_heads;
+    it.nt = max(1, (r.cap - it.lo + kKv8Group - 1) / kKv8Group);  // a sequence without tokens still gets its rows written
+    const long long units = (long long)it.rt * it.nt * p.c.n_kv_heads;
+    it.units = (int)min(units, (long long)INT_MAX);
     return it;
 }
+
+// Run of CTA c when `total` units are cut into `ctas` runs, and the CTA that has unit u.
+struct Cut {
+    int q, rem;  // units of a run, and how many runs have one more
+    IAM_DEV int first(int c) const { return q * c + min(c, rem); }
+    IAM_DEV int owner(int u) const {
+        const int big = rem * (q + 1);
+        return u < big ? u / (q + 1) : rem + (u - big) / q;
+    }
+};
 
 // C += A B with A a 16 x 16 tile; the transpose of an 8 x 8 tile of 16-bit values across the warp.
 IAM_DEV uint32_t transpose8(uint32_t v) {
@@ -46,37 +69,58 @@ IAM_DEV uint32_t transpose8(uint32_t v) {
 
 // T: query and output type; TERMS 2 (fp32): columns 0..3 of the tile hold the rows' high fp16 terms and
 // 4..7 the low ones (and so for the probabilities), which carries 22 bits of both through fp16 products.
+// Each warp streams its own groups of tokens through its own ring in shared memory: lane 0 has TMA fetch a group's
+// keys and values (16 rows each, swizzled so that the reads below meet no bank twice) as soon as the warp has
+// taken the group before out of that place; no warp waits for another.  The fragments' rows are tokens in the
+// order 0 4 2 6 5 1 7 3 for the same reason: eight lanes then read eight different 16-byte columns both as
+// keys (two tokens, four columns) and as values (four tokens, two columns).
 template <class T, int FMT, int HD, int TERMS>
-__global__ void __launch_bounds__(kThreads) kv8_decode_kernel(Kv8Attn p) {
-    constexpr int RT = 8 / TERMS;
+__global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
+    kv8_decode_kernel(const Kv8Attn p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    using S = Shape<HD>;
+    constexpr int RT = 8 / TERMS, W = S::kWarps;
     constexpr int KS = HD / 16, KL = HD / 64, VW = HD / 32, MT = HD / 16;
-    constexpr int PITCH = HD + 4;
-    __shared__ __align__(16) float s_o[kWarps][8][PITCH];
-    __shared__ float s_m[kWarps][8], s_l[kWarps][8];
+    constexpr int PITCH = S::kPitch;
+    extern __shared__ unsigned char s_raw[];
+    __shared__ __align__(8) uint64_t s_full[W][S::kStages];
+    __shared__ float s_m[W][8], s_l[W][8];
     __shared__ float s_top[8], s_sum[8];
     __shared__ int s_last;
+    unsigned char* ring = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
+    auto s_o = reinterpret_cast<float (*)[8][PITCH]>(ring);  // the warps' results, when the codes are used up
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tig = lane & 3;
     const int plog = 31 - __clz(p.c.page_size), kvh = p.c.n_kv_heads;
+    unsigned char* mine_ring = ring + (size_t)warp * S::kStages * S::kStage;
+    if (lane == 0) {
+        for (int i = 0; i < S::kStages; ++i) mbar_init(&s_full[warp][i], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
 
     // ---- this CTA's run of units (every warp finds it by itself)
-    long long total = 0;
+    long long all = 0;
     for (int i = lane; i < p.c.n_seqs; i += 32)
-        total += item_of<RT>(p, seq_rows(p.c, p.cu, p.lens, p.n_rows, i, blockIdx.x == 0 ? p.s.err : nullptr)).units;
+        all += item_of<RT>(p, seq_rows(p.c, p.cu, p.lens, p.n_rows, i, blockIdx.x == 0 && warp == 0 ? p.s.err : nullptr)).units;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (total == 0) return;
-    const long long ctas = min((long long)gridDim.x, (total + kMinUnits - 1) / kMinUnits);
-    if (blockIdx.x >= ctas) return;
-    const long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
-    long long base = 0;  // units before sequence `seq`
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (all == 0) return;
+    if (all > INT_MAX / 2) {  // (more than 16 G tokens)
+        if (blockIdx.x == 0 && tid == 0) atomicOr(p.s.err, kKv8ErrRange);
+        return;
+    }
+    const int total = (int)all, ctas = min((int)gridDim.x, (total + kMinUnits - 1) / kMinUnits);
+    if ((int)blockIdx.x >= ctas) return;
+    const Cut cut{total / ctas, total % ctas};
+    const int u0 = cut.first(blockIdx.x), u1 = cut.first(blockIdx.x + 1);
+    int base = 0;  // units before sequence `seq`
     int seq = 0;
-    for (int i0 = 0;; i0 += 32) {
-        long long mine = 0;
+    for (int i0 = 0; p.c.n_seqs > 1; i0 += 32) {
+        int mine = 0;
         if (i0 + lane < p.c.n_seqs) mine = item_of<RT>(p, seq_rows(p.c, p.cu, p.lens, p.n_rows, i0 + lane, nullptr)).units;
-        long long sum = mine;
+        int sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long up = __shfl_up_sync(0xffffffffu, sum, o);
+            const int up = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += up;
         }
         const unsigned past = __ballot_sync(0xffffffffu, base + sum > u0);
@@ -89,7 +133,8 @@ __global__ void __launch_bounds__(kThreads) kv8_decode_kernel(Kv8Attn p) {
         base += __shfl_sync(0xffffffffu, sum, 31);
     }
 
-    long long u = u0;
+    uint32_t phases = 0;  // of the ring's barriers, a bit each
+    int u = u0;
     while (u < u1) {
         SeqRows r = seq_rows(p.c, p.cu, p.lens, p.n_rows, seq, nullptr);
         Item it = item_of<RT>(p, r);
@@ -99,83 +144,55 @@ __global__ void __launch_bounds__(kThreads) kv8_decode_kernel(Kv8Attn p) {
             r = seq_rows(p.c, p.cu, p.lens, p.n_rows, seq, nullptr);
             it = item_of<RT>(p, r);
         }
-        const long long rel = u - base;
-        const int tile = (int)(rel % it.nt), rth = (int)(rel / it.nt);
+        const int rel = u - base;
+        const int rth = rel / it.nt, tile = rel - rth * it.nt;
         const int head = rth / it.rt, rtile = rth - head * it.rt;
-        const long long item0 = u - tile, item1 = item0 + it.nt;
-        const long long seg_end = min(u1, item1);
-        const int t0 = it.lo + tile * kTile, t1 = min(r.cap, t0 + (int)(seg_end - u) * kTile);
+        const int item0 = u - tile, item1 = item0 + it.nt;
+        const int seg_end = min(u1, item1);
+        const int t0 = it.lo + tile * kKv8Group, t1 = min(r.cap, t0 + (seg_end - u) * kKv8Group);
         const int n_rows = min(RT, r.n * p.gq - rtile * RT);  // rows of this tile
         const int pos_lo = r.start + rtile * RT / p.gq, pos_hi = r.start + (rtile * RT + n_rows - 1) / p.gq;
 
-        // ---- this warp's groups of 16 tokens: t0 + 16 (warp + kWarps i), i < cnt
+        // ---- this warp's groups of 16 tokens: t0 + 16 (warp + W i), i < cnt
+        constexpr int STRIDE = W * kKv8Group;
         const int first = t0 + warp * kKv8Group;
-        const int cnt = first < t1 ? (t1 - first + kTile - 1) / kTile : 0;
+        const int cnt = first < t1 ? (t1 - first + STRIDE - 1) / STRIDE : 0;
         const int32_t* table = p.c.block_table + (size_t)seq * p.c.max_pages;
-        // lane l keeps page and scales of group (i & ~31) + l
-        int ids = -1;
-        float kss = 0.0f, vss = 0.0f;
+        // lane l keeps the page of group (i & ~31) + l, looked up when the copies get there, and its scales
+        int ids = -1, ids_before = -1;
+        float kss = 0.0f, vss = 0.0f, kss_before = 0.0f, vss_before = 0.0f;
         auto look_up = [&](int i) {
-            const int t = first + (i + lane) * kTile;
+            const int t = first + (i + lane) * STRIDE;
+            ids_before = ids;
+            kss_before = kss;
+            vss_before = vss;
             ids = -1;
             if (t < t1) {
                 ids = table[t >> plog];
                 if (ids < 0 || ids >= p.c.n_pages) {
-                    *p.s.err = 1u;
+                    atomicOr(p.s.err, kKv8ErrRange);
                     ids = -1;
                 }
             }
             kss = ids >= 0 ? p.c.k_scale[(size_t)ids * kvh + head] : 0.0f;
             vss = ids >= 0 ? p.c.v_scale[(size_t)ids * kvh + head] : 0.0f;
         };
-        uint4 kq[2][KL];
-        uint32_t vq[4][VW];
-        auto row_at = [&](const void* codes, int id, int t) {
-            return static_cast<const uint8_t*>(codes) + ((((size_t)id * kvh + head) << plog) + (t & (p.c.page_size - 1))) * HD;
-        };
-        auto load_k = [&](int id, int t) {
+        auto issue = [&](int i) {  // group i into stage i % kStages
+            if ((i & 31) == 0) look_up(i);
+            const int id = __shfl_sync(0xffffffffu, ids, i & 31);
+            if (lane == 0 && id >= 0) {
+                const int t = first + i * STRIDE, st = i % S::kStages;
+                const int row = (int)((((long long)id * kvh + head) << plog) + (t & (p.c.page_size - 1)));
+                unsigned char* to = mine_ring + st * S::kStage;
+                mbar_expect_tx(&s_full[warp][st], S::kStage);
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int c = 0; c < KL; ++c) kq[half][c] = make_uint4(0u, 0u, 0u, 0u);
-            if (id < 0) return;
-            const uint8_t* src = row_at(p.c.k, id, t) + g * HD + tig * 16;
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int c = 0; c < KL; ++c) kq[half][c] = __ldcs(reinterpret_cast<const uint4*>(src + half * 8 * HD + c * 64));
-        };
-        auto load_v = [&](int id, int t) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int tok = 2 * tig + (j & 1) + (j >> 1) * 8;
-#pragma unroll
-                for (int c = 0; c < VW; ++c) vq[j][c] = 0u;
-                if (id < 0 || t + tok >= r.cap) continue;  // what is behind the last token is not read
-                const uint8_t* src = row_at(p.c.v, id, t) + tok * HD;
-                if constexpr (VW == 2) {
-                    const uint2 w = __ldcs(reinterpret_cast<const uint2*>(src + g * 8));
-                    vq[j][0] = w.x;
-                    vq[j][1] = w.y;
-                } else {
-#pragma unroll
-                    for (int c = 0; c < VW / 4; ++c) {
-                        const uint4 w = __ldcs(reinterpret_cast<const uint4*>(src + c * 128 + g * 16));
-                        vq[j][4 * c] = w.x;
-                        vq[j][4 * c + 1] = w.y;
-                        vq[j][4 * c + 2] = w.z;
-                        vq[j][4 * c + 3] = w.w;
-                    }
+                for (int h = 0; h < S::kHalves; ++h) {
+                    tma_load_2d(to + h * S::kBox, &map_k, 128 * h, row, &s_full[warp][st]);
+                    tma_load_2d(to + (S::kHalves + h) * S::kBox, &map_v, 128 * h, row, &s_full[warp][st]);
                 }
             }
         };
-        int id = -1;
-        if (cnt > 0) {
-            look_up(0);
-            id = __shfl_sync(0xffffffffu, ids, 0);
-            load_k(id, first);
-            load_v(id, first);
-        }
+        for (int i = 0; i < min(cnt, S::kStages); ++i) issue(i);
 
         // ---- queries: column g's fragment; dims 64 c + 16 tig + 4 w + {0, 1} and {2, 3} are k-step
         // 4 c + w's columns 2 tig + {0, 1} and + 8
@@ -227,26 +244,72 @@ __global__ void __launch_bounds__(kThreads) kv8_decode_kernel(Kv8Attn p) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[mt][e] = 0.0f;
 
+        // fragment row j is token order[j] of its eight
+        auto token = [](int j) { return HD == 64 ? j : (0x37156240 >> (4 * j)) & 7; };
+        // the 16-byte column c of a row in the swizzled box
+        auto column = [](int row, int c) {
+            return HD == 64 ? row * 64 + ((c ^ ((row >> 1) & 3)) << 4) : row * 128 + ((c ^ (row & 7)) << 4);
+        };
+        const int tok_g = token(g);
         for (int i = 0; i < cnt; ++i) {
-            const int t = first + i * kTile;
-            const float ks_now = __shfl_sync(0xffffffffu, kss, i & 31), vs_now = __shfl_sync(0xffffffffu, vss, i & 31);
+            const int t = first + i * STRIDE, st = i % S::kStages;
+            // (the copies may already be a batch of 32 look-ups further)
+            const bool older = (i & ~31) != (min(i + S::kStages - 1, cnt - 1) & ~31);
+            const int id = __shfl_sync(0xffffffffu, older ? ids_before : ids, i & 31);
+            const float ks_now = __shfl_sync(0xffffffffu, older ? kss_before : kss, i & 31);
+            const float vs_now = __shfl_sync(0xffffffffu, older ? vss_before : vss, i & 31);
             const bool bad = id < 0;
-            // scores of tokens g and g + 8 (rows), columns 2 tig and 2 tig + 1
-            float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const uint32_t w0 = reinterpret_cast<const uint32_t*>(&kq[0][ks >> 2])[ks & 3];
-                const uint32_t w1 = reinterpret_cast<const uint32_t*>(&kq[1][ks >> 2])[ks & 3];
-                uint32_t a[4];
-                codes_to_half<FMT>(w0, a[0], a[2]);
-                codes_to_half<FMT>(w1, a[1], a[3]);
-                mma_16816(sc, a, bq[ks][0], bq[ks][1]);
+            const unsigned char* box_k = mine_ring + st * S::kStage;
+            const unsigned char* box_v = box_k + S::kHalves * S::kBox;
+            if (!bad) {
+                if (!mbar_wait(&s_full[warp][st], (phases >> st) & 1u, nullptr)) atomicOr(p.s.err, kKv8ErrWait);
+                phases ^= 1u << st;
             }
-            int id_next = -1;
-            if (i + 1 < cnt) {
-                if (((i + 1) & 31) == 0) look_up(i + 1);
-                id_next = __shfl_sync(0xffffffffu, ids, (i + 1) & 31);
-                load_k(id_next, t + kTile);
+            // scores of fragment rows g and g + 8, columns 2 tig and 2 tig + 1
+            float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sd[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < KL; ++c) {
+                const unsigned char* half = box_k + (HD == 256 ? (c >> 1) * S::kBox : 0);
+                const int piece = HD == 256 ? (c & 1) * 4 + tig : c * 4 + tig;
+                const uint4 q0 = *reinterpret_cast<const uint4*>(half + column(tok_g, piece));
+                const uint4 q1 = *reinterpret_cast<const uint4*>(half + column(tok_g + 8, piece));
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t a[4];
+                    codes_to_half<FMT>(reinterpret_cast<const uint32_t*>(&q0)[w], a[0], a[2]);
+                    codes_to_half<FMT>(reinterpret_cast<const uint32_t*>(&q1)[w], a[1], a[3]);
+                    mma_16816(w & 1 ? sd : sc, a, bq[4 * c + w][0], bq[4 * c + w][1]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[e] += sd[e];
+            uint32_t vq[4][VW];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int tok = token(2 * tig + (j & 1)) + (j >> 1) * 8;
+                if constexpr (VW == 2) {
+                    const uint2 w = *reinterpret_cast<const uint2*>(box_v + column(tok, g >> 1) + (g & 1) * 8);
+                    vq[j][0] = w.x;
+                    vq[j][1] = w.y;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < VW / 4; ++c) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(box_v + c * S::kBox + column(tok, g));
+                        vq[j][4 * c] = w.x;
+                        vq[j][4 * c + 1] = w.y;
+                        vq[j][4 * c + 2] = w.z;
+                        vq[j][4 * c + 3] = w.w;
+                    }
+                }
+            }
+            __syncwarp();
+            if (i + S::kStages < cnt) issue(i + S::kStages);
+            if (t + kKv8Group > r.cap || bad) {  // what stands behind the last token has no part in the sums
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (bad || t + token(2 * tig + (j & 1)) + (j >> 1) * 8 >= r.cap)
+#pragma unroll
+                        for (int c = 0; c < VW; ++c) vq[j][c] = 0u;
             }
             if (TERMS == 2)
 #pragma unroll
@@ -259,7 +322,7 @@ __global__ void __launch_bounds__(kThreads) kv8_decode_kernel(Kv8Attn p) {
                 const float f = fminf(ks_now * rf[h], 3.402823466e38f);
                 float s0 = sc[h] * f, s1 = sc[2 + h] * f;
                 if (!whole) {
-                    const int ta = t + g, tb = ta + 8;
+                    const int ta = t + tok_g, tb = ta + 8;
                     if (bad || ta > pos[h] || ta >= r.cap || (p.window > 0 && ta <= pos[h] - p.window)) s0 = -INFINITY;
                     if (bad || tb > pos[h] || tb >= r.cap || (p.window > 0 && tb <= pos[h] - p.window)) s1 = -INFINITY;
                 }
@@ -279,7 +342,7 @@ __global__ void __launch_bounds__(kThreads) kv8_decode_kernel(Kv8Attn p) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sc[e] = split_lo(sc[e]);
             const uint32_t b0 = transpose8(pack_h2(sc[0], sc[1])), b1 = transpose8(pack_h2(sc[2], sc[3]));
-            // values: word c of tokens 2 tig, 2 tig + 1 (a, b) and + 8 (cc, d) makes m-tiles 2 c and 2 c + 1,
+            // values: word c of fragment columns 2 tig, 2 tig + 1 (a, b) and + 8 (cc, d) makes m-tiles 2 c and 2 c + 1,
             // whose rows g and g + 8 are dims 4 c' + {0, 1} and {2, 3} of this lane's piece
 #pragma unroll
             for (int c = 0; c < VW; ++c) {
@@ -300,11 +363,10 @@ __global__ void __launch_bounds__(kThreads) kv8_decode_kernel(Kv8Attn p) {
                     om[3] = fmaf(acc[3], vs_now, om[3] * rescale[1]);
                 }
             }
-            if (i + 1 < cnt) load_v(id_next, t + kTile);
-            id = id_next;
         }
 
         // ---- join the warps in warp order
+        __syncthreads();  // every warp's codes are used up
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
@@ -326,16 +388,16 @@ __global__ void __launch_bounds__(kThreads) kv8_decode_kernel(Kv8Attn p) {
         __syncthreads();
         const bool complete = tile == 0 && seg_end == item1;
         // CTAs that share this row tile: the owner of its first unit to the owner of its last
-        const int cta0 = (int)(((item0 + 1) * ctas - 1) / total), cta1 = (int)((item1 * ctas - 1) / total);
+        const int cta0 = cut.owner(item0), cta1 = cut.owner(item1 - 1);
         float* part = p.s.part + (size_t)(2 * blockIdx.x + ((int)blockIdx.x == cta0 ? 1 : 0)) * 8 * PITCH;
-        for (int e = tid; e < n_rows * HD; e += kThreads) {
+        for (int e = tid; e < n_rows * HD; e += S::kThreads) {
             const int col = e / HD, d = e - col * HD;
             float top = -INFINITY, sum = 0.0f, acc = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][col]);
+            for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w][col]);
             const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
+            for (int w = 0; w < W; ++w) {
                 const float f = ex2(s_m[w][col] - ref);
                 sum = fmaf(f, s_l[w][col], sum);
                 float v = s_o[w][col][d];
@@ -365,7 +427,7 @@ __global__ void __launch_bounds__(kThreads) kv8_decode_kernel(Kv8Attn p) {
                 __threadfence();
                 const int parts = cta1 - cta0 + 1;
                 auto part_of = [&](int k) { return p.s.part + (size_t)(2 * (cta0 + k) + (k == 0 ? 1 : 0)) * 8 * PITCH; };
-                for (int col = warp; col < n_rows; col += kWarps) {
+                for (int col = warp; col < n_rows; col += W) {
                     float top = -INFINITY;
                     for (int k = lane; k < parts; k += 32) top = fmaxf(top, __ldcg(part_of(k) + col * PITCH + HD));
                     top = warp_max(top);
@@ -381,11 +443,11 @@ __global__ void __launch_bounds__(kThreads) kv8_decode_kernel(Kv8Attn p) {
                     }
                 }
                 __syncthreads();
-                for (int e = tid; e < n_rows * (HD / 4); e += kThreads) {
+                for (int e = tid; e < n_rows * (HD / 4); e += S::kThreads) {
                     const int col = e / (HD / 4), d = (e - col * (HD / 4)) * 4;
                     const float ref = s_top[col] == -INFINITY ? 0.0f : s_top[col];
                     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+#pragma unroll 8
                     for (int k = 0; k < parts; ++k) {
                         const float* from = part_of(k) + col * PITCH;
                         const float f = ex2(__ldcg(from + HD) - ref);
@@ -407,21 +469,39 @@ __global__ void __launch_bounds__(kThreads) kv8_decode_kernel(Kv8Attn p) {
                 if (tid == 0) p.s.ctr[cta0] = 0;  // ready for the next call
             }
         }
-        __syncthreads();  // shared memory is reused by the next segment
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring is the copies' again
+        __syncthreads();
         u = seg_end;
     }
 }
 
+// The cache's codes as rows of head_dim bytes, copied 16 rows (of at most 128 bytes) at a time.
+template <int HD>
+int make_map(CUtensorMap* map, const void* codes, const iam_kv8_cache& c) {
+    auto fn = tensor_map_encoder();
+    if (fn == nullptr) return fail(IAM_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[2] = {HD, (cuuint64_t)c.n_pages * c.n_kv_heads * c.page_size};
+    const cuuint64_t strides[1] = {HD};
+    const cuuint32_t box[2] = {HD > 128 ? 128 : HD, kKv8Group};
+    const cuuint32_t estr[2] = {1u, 1u};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, HD == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(IAM_ERR_CUDA, "kv8: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+    return IAM_OK;
+}
+
 template <class T, int FMT, int HD>
 int launch(const Kv8Attn& a, cudaStream_t s) {
+    constexpr size_t smem = Shape<HD>::kRing + 1024;
     auto kern = kv8_decode_kernel<T, FMT, HD, sizeof(T) == 4 ? 2 : 1>;
-    static std::atomic<int> resident{0};
-    int n = resident.load(std::memory_order_relaxed);
-    if (n == 0) {
-        IAM_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, kThreads, 0));
-        resident.store(n, std::memory_order_relaxed);
-    }
-    kern<<<std::min(a.s.max_ctas, n * a.sms), kThreads, 0, s>>>(a);
+    static std::atomic<unsigned long long> done{0};
+    IAM_CUDA_TRY(once_per_device(done, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }));
+    CUtensorMap mk, mv;
+    int rc = make_map<HD>(&mk, a.c.k, a.c);
+    if (rc == IAM_OK) rc = make_map<HD>(&mv, a.c.v, a.c);
+    if (rc) return rc;
+    kern<<<a.sms, Shape<HD>::kThreads, smem, s>>>(a, mk, mv);
     IAM_CUDA_TRY(cudaGetLastError());
     return IAM_OK;
 }
@@ -436,6 +516,9 @@ int launch_dim(const Kv8Attn& a, cudaStream_t s) {
 }
 
 }  // namespace
+
+int kv8_max_ctas(int sms) { return 4 * sms; }
+size_t kv8_decode_part_floats(int head_dim, int sms) { return (size_t)2 * sms * 8 * (head_dim + 4); }
 
 int kv8_decode_launch(const Kv8Attn& a, int dtype, cudaStream_t s) {
     return with_dtype(dtype, [&](auto t) {

@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(Kv8Attn p) {
                 int id = -1;
                 if (t < r.cap) id = __ldg(table + (t >> plog));
                 if (id < 0 || id >= p.c.n_pages) {
-                    if (t < r.cap) *p.s.err = 1u;
+                    if (t < r.cap) atomicOr(p.s.err, kKv8ErrRange);
                     id = -1;
                 }
                 if (c == 0 && (row & (kKv8Group - 1)) == 0) {
@@ -470,12 +470,8 @@ int launch_dim(const Kv8Attn& a, cudaStream_t s) {
 
 }  // namespace
 
-int kv8_max_ctas(int sms) { return 16 * sms; }
 size_t kv8_plan_words() { return 2 + 3 * (size_t)kKv8MaxItems; }
-size_t kv8_part_floats(int head_dim, int sms) {
-    const size_t pitch = head_dim + 4;
-    return std::max((size_t)2 * kv8_max_ctas(sms) * 8 * pitch, (size_t)2 * kPerSm * sms * kRows * pitch);
-}
+size_t kv8_rows_part_floats(int head_dim, int sms) { return (size_t)2 * kPerSm * sms * kRows * (head_dim + 4); }
 
 int kv8_rows_launch(const Kv8Attn& a, int dtype, cudaStream_t s) {
     if ((long long)a.n_rows * a.gq / kRows + a.c.n_seqs > kKv8MaxItems)
