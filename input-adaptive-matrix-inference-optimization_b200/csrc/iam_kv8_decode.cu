@@ -5,9 +5,10 @@
 // or the dims (for the values) its M, so a code enters one MMA and no row of the tile is padding for
 // want of queries.  Which physical dim plays a fragment's k (scores) or row (values) is free as long as the
 // queries and the output agree: the choice below makes every access 16 bytes of adjacent codes of one token.
-#include <climits>
 #include <algorithm>
 #include <atomic>
+#include <climits>
+#include <type_traits>
 
 #include "iam_kv8.cuh"
 #include "iam_tc.cuh"
@@ -15,9 +16,11 @@
 namespace iam {
 namespace {
 
-constexpr int kMinUnits = 8;  // work units of a CTA at least, while there are enough
+constexpr int kMinGroups = 8;  // groups of tokens of a CTA at least, where a context is shared
+constexpr int kItemCost = 24;  // what opening and joining a piece of a context costs, in groups
 
-// Warps of a CTA (one CTA an SM) and groups of 16 tokens in each warp's ring: 192 KB of codes on their way.
+// Warps of a CTA (one CTA an SM; one warp more feeds them) and groups of 16 tokens in each warp's ring: 128 KB of
+// codes on their way.
 template <int HD>
 struct Shape {
     static constexpr int kWarps = HD == 256 ? 8 : 16;
@@ -25,32 +28,36 @@ struct Shape {
     static constexpr int kHalves = HD == 256 ? 2 : 1;          // 128-byte columns of a row
     static constexpr int kBox = kKv8Group * HD / kHalves;      // bytes of one copy
     static constexpr int kStage = 2 * kHalves * kBox;          // a group's keys and values
-    static constexpr int kStages = 192 * 1024 / (kWarps * kStage);
+    static constexpr int kStages = 128 * 1024 / (kWarps * kStage);
     static constexpr int kRing = kWarps * kStages * kStage;
     static constexpr int kPitch = HD + 4;
-    static_assert(kWarps * 8 * kPitch * 4 <= kRing, "the warps' results are joined where the codes were");
+    static constexpr int kHeads = HD == 256 ? 4 : 8;            // heads of an item at most
+    static constexpr int kSmem = kRing + kWarps * 8 * kPitch * 4 + 1024;
 };
 
-// The call's work: groups of 16 tokens in the order (sequence, KV head, row tile, token), cut into equal runs, one
-// per CTA, whatever the sequences' lengths.
-struct Item {
-    int rt, nt;    // row tiles of the sequence, groups of one
-    int lo;        // first token read (a multiple of kKv8Group)
-    int units;     // of the whole sequence (the sum over the sequences is checked against 2^31)
+// A (sequence, group of `hg` KV heads, row tile) is an item: nt groups of 16 tokens from token lo on, of each of its
+// heads; a CTA's warps are dealt to the heads.  (One head an item while items are fewer than SMs; more
+// where there are many, for a piece's opening and join are paid once for all of its heads.)  Items are laid end to
+// end, each preceded by kItemCost groups of nothing, and the line is cut into equal runs, one per CTA, whatever
+// the sequences' lengths.  With at most half as many items as SMs each gets CTAs of its own in proportion, so
+// that none opens a second piece.
+struct Items {
+    int n;   // items of the sequence
+    int rt;  // row tiles of a group of heads
+    int nt, lo;
 };
 
 template <int RT>
-IAM_DEV Item item_of(const Kv8Attn& p, const SeqRows& r) {
-    Item it;
+IAM_DEV Items items_of(const Kv8Attn& p, int hg, const SeqRows& r) {
+    Items it;
     it.rt = (r.n * p.gq + RT - 1) / RT;
+    it.n = (int)min((long long)it.rt * (p.c.n_kv_heads / hg), (long long)INT_MAX);
     it.lo = p.window > 0 ? max(0, r.start - p.window + 1) & ~(kKv8Group - 1) : 0;
     it.nt = max(1, (r.cap - it.lo + kKv8Group - 1) / kKv8Group);  // a sequence without tokens still gets its rows written
-    const long long units = (long long)it.rt * it.nt * p.c.n_kv_heads;
-    it.units = (int)min(units, (long long)INT_MAX);
     return it;
 }
 
-// Run of CTA c when `total` units are cut into `ctas` runs, and the CTA that has unit u.
+// The line of `total` units cut into `ctas` runs: the first unit of CTA c's, and the CTA that has unit u.
 struct Cut {
     int q, rem;  // units of a run, and how many runs have one more
     IAM_DEV int first(int c) const { return q * c + min(c, rem); }
@@ -59,6 +66,12 @@ struct Cut {
         return u < big ? u / (q + 1) : rem + (u - big) / q;
     }
 };
+
+IAM_DEV long long warp_sum(long long v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
 
 // C += A B with A a 16 x 16 tile; the transpose of an 8 x 8 tile of 16-bit values across the warp.
 IAM_DEV uint32_t transpose8(uint32_t v) {
@@ -69,172 +82,274 @@ IAM_DEV uint32_t transpose8(uint32_t v) {
 
 // T: query and output type; TERMS 2 (fp32): columns 0..3 of the tile hold the rows' high fp16 terms and
 // 4..7 the low ones (and so for the probabilities), which carries 22 bits of both through fp16 products.
-// Each warp streams its own groups of tokens through its own ring in shared memory: lane 0 has TMA fetch a group's
-// keys and values (16 rows each, swizzled so that the reads below meet no bank twice) as soon as the warp has
-// taken the group before out of that place; no warp waits for another.  The fragments' rows are tokens in the
-// order 0 4 2 6 5 1 7 3 for the same reason: eight lanes then read eight different 16-byte columns both as
-// keys (two tokens, four columns) and as values (four tokens, two columns).
+// Each warp has a ring of its own in shared memory, and lane w of the feeding warp keeps warp w's full: it has TMA
+// fetch a group's keys and values (16 rows each, swizzled so that the reads below meet no bank twice) as soon as
+// the warp has taken an earlier group out of that place, into the next piece of context already; the warps
+// wait for one another only to join a piece's results.  The fragments' rows are tokens in the order
+// 0 4 2 6 5 1 7 3 for the same reason: eight lanes then read eight different 16-byte columns both as keys (two
+// tokens, four columns) and as values (four tokens, two columns).
 template <class T, int FMT, int HD, int TERMS>
-__global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
-    kv8_decode_kernel(const Kv8Attn p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+__global__ void __launch_bounds__(Shape<HD>::kThreads + 32, 1)
+    kv8_decode_kernel(const Kv8Attn p, int hg, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
     using S = Shape<HD>;
     constexpr int RT = 8 / TERMS, W = S::kWarps;
     constexpr int KS = HD / 16, KL = HD / 64, VW = HD / 32, MT = HD / 16;
-    constexpr int PITCH = S::kPitch;
+    constexpr int PITCH = S::kPitch, QE = HD / 32;
     extern __shared__ unsigned char s_raw[];
-    __shared__ __align__(8) uint64_t s_full[W][S::kStages];
+    __shared__ __align__(8) uint64_t s_full[W][S::kStages], s_free[W][S::kStages];
+    __shared__ float4 s_group[W][S::kStages];  // key scale, value scale, page (as bits) of the group in a place
+    __shared__ __align__(16) __half s_q[S::kHeads][8][HD + 8];  // [head of the item][column]
+    __shared__ float s_rf[S::kHeads][8];
     __shared__ float s_m[W][8], s_l[W][8];
-    __shared__ float s_top[8], s_sum[8];
+    __shared__ float s_weight[W][8], s_top[S::kHeads][8], s_sum[S::kHeads][8];
     __shared__ int s_last;
     unsigned char* ring = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
-    auto s_o = reinterpret_cast<float (*)[8][PITCH]>(ring);  // the warps' results, when the codes are used up
+    auto s_o = reinterpret_cast<float (*)[8][PITCH]>(ring + S::kRing);  // the warps' results
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tig = lane & 3;
     const int plog = 31 - __clz(p.c.page_size), kvh = p.c.n_kv_heads;
-    unsigned char* mine_ring = ring + (size_t)warp * S::kStages * S::kStage;
-    if (lane == 0) {
-        for (int i = 0; i < S::kStages; ++i) mbar_init(&s_full[warp][i], 1);
+    const int per_head = W / hg;  // warps that share a head
+    if (tid < W) {
+        for (int i = 0; i < S::kStages; ++i) {
+            mbar_init(&s_full[tid][i], 1);
+            mbar_init(&s_free[tid][i], 1);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    __syncwarp();
+    if (tid == W) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+    }
+    __syncthreads();
 
-    // ---- this CTA's run of units (every warp finds it by itself)
-    long long all = 0;
-    for (int i = lane; i < p.c.n_seqs; i += 32)
-        all += item_of<RT>(p, seq_rows(p.c, p.cu, p.lens, p.n_rows, i, blockIdx.x == 0 && warp == 0 ? p.s.err : nullptr)).units;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-    if (all == 0) return;
-    if (all > INT_MAX / 2) {  // (more than 16 G tokens)
+    // ---- this CTA's run (every warp finds it by itself)
+    long long n_items = 0, n_groups = 0;
+    for (int i = lane; i < p.c.n_seqs; i += 32) {
+        const Items it = items_of<RT>(p, hg, seq_rows(p.c, p.cu, p.lens, p.n_rows, i, blockIdx.x == 0 && warp == 0 ? p.s.err : nullptr));
+        n_items += it.n;
+        n_groups += (long long)it.n * it.nt;
+    }
+    n_items = warp_sum(n_items);
+    n_groups = warp_sum(n_groups);
+    if (n_items == 0) return;
+    const long long line = n_groups + n_items * kItemCost;
+    if (line > INT_MAX / 2) {  // (more than 16 G tokens)
         if (blockIdx.x == 0 && tid == 0) atomicOr(p.s.err, kKv8ErrRange);
         return;
     }
-    const int total = (int)all, ctas = min((int)gridDim.x, (total + kMinUnits - 1) / kMinUnits);
-    if ((int)blockIdx.x >= ctas) return;
+    const int grid = gridDim.x;
+    const bool few = n_items * 2 <= grid;
+    // few: the CTAs that share an item, so that their sum over the items is at most the grid
+    auto sharers = [&](const Items& it) {
+        return min(1 + (int)((long long)it.nt * (grid - n_items) / n_groups), (it.nt + kMinGroups - 1) / kMinGroups);
+    };
+    const int total = (int)line, ctas = min(grid, (int)min((n_groups + kMinGroups - 1) / kMinGroups, (long long)grid));
+    if (!few && (int)blockIdx.x >= ctas) return;
     const Cut cut{total / ctas, total % ctas};
-    const int u0 = cut.first(blockIdx.x), u1 = cut.first(blockIdx.x + 1);
-    int base = 0;  // units before sequence `seq`
-    int seq = 0;
+    const int u0 = few ? (int)blockIdx.x : cut.first(blockIdx.x), u1 = few ? u0 + 1 : cut.first(blockIdx.x + 1);
+    int base0 = 0, seq0 = 0;  // what stands before sequence seq0: CTAs (few) or units
     for (int i0 = 0; p.c.n_seqs > 1; i0 += 32) {
         int mine = 0;
-        if (i0 + lane < p.c.n_seqs) mine = item_of<RT>(p, seq_rows(p.c, p.cu, p.lens, p.n_rows, i0 + lane, nullptr)).units;
+        if (i0 + lane < p.c.n_seqs) {
+            const Items it = items_of<RT>(p, hg, seq_rows(p.c, p.cu, p.lens, p.n_rows, i0 + lane, nullptr));
+            mine = it.n * (few ? sharers(it) : it.nt + kItemCost);
+        }
         int sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int up = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += up;
         }
-        const unsigned past = __ballot_sync(0xffffffffu, base + sum > u0);
+        const unsigned past = __ballot_sync(0xffffffffu, base0 + sum > u0);
         if (past) {
             const int at = __ffs(past) - 1;
-            base += __shfl_sync(0xffffffffu, sum - mine, at);
-            seq = i0 + at;
+            base0 += __shfl_sync(0xffffffffu, sum - mine, at);
+            seq0 = i0 + at;
             break;
         }
-        base += __shfl_sync(0xffffffffu, sum, 31);
+        base0 += __shfl_sync(0xffffffffu, sum, 31);
+        if (i0 + 32 >= p.c.n_seqs) return;  // (few: more CTAs than shares)
     }
 
-    uint32_t phases = 0;  // of the ring's barriers, a bit each
-    int u = u0;
-    while (u < u1) {
-        SeqRows r = seq_rows(p.c, p.cu, p.lens, p.n_rows, seq, nullptr);
-        Item it = item_of<RT>(p, r);
-        while (u >= base + it.units) {  // (sequences without rows have no units)
-            base += it.units;
-            ++seq;
-            r = seq_rows(p.c, p.cu, p.lens, p.n_rows, seq, nullptr);
-            it = item_of<RT>(p, r);
+    // A piece of an item: groups [ta, tb) of it, shared by CTAs cta0 .. cta1.  The feeding lanes walk the pieces
+    // ahead of the warps.
+    struct Piece {
+        int u, base, seq;  // place on the line, units (or CTAs) before the sequence
+        SeqRows r;
+        int head, rtile, ta, tb, lo, cta0, cta1;  // head: the first of its group
+    };
+    auto open = [&](Piece& c) {  // the piece at c.u < u1; advances c.u behind it
+        for (;;) {
+            c.r = seq_rows(p.c, p.cu, p.lens, p.n_rows, c.seq, nullptr);
+            const Items it = items_of<RT>(p, hg, c.r);
+            const int share = few ? sharers(it) : it.nt + kItemCost, end = c.base + it.n * share;
+            if (c.u >= end) {  // (sequences without rows have no items)
+                c.base = end;
+                if (++c.seq >= p.c.n_seqs) {
+                    c.u = u1;
+                    c.ta = c.tb = 0;
+                    return false;
+                }
+                continue;
+            }
+            const int rel = c.u - c.base, item = rel / share, idx = rel - item * share;
+            c.lo = it.lo;
+            c.head = item / it.rt;
+            c.rtile = item - c.head * it.rt;
+            c.head *= hg;
+            const int item0 = c.u - idx;
+            if (few) {
+                c.ta = (int)((long long)it.nt * idx / share);
+                c.tb = (int)((long long)it.nt * (idx + 1) / share);
+                c.cta0 = item0;
+                c.cta1 = item0 + share - 1;
+                ++c.u;
+                return true;
+            }
+            const int stop = min(u1, item0 + share);
+            c.ta = max(0, idx - kItemCost);
+            c.tb = max(0, stop - item0 - kItemCost);
+            c.cta0 = cut.owner(item0 + kItemCost);
+            c.cta1 = cut.owner(item0 + share - 1);
+            c.u = stop;
+            if (c.tb > c.ta) return true;
+            if (c.u >= u1) return false;  // nothing of the item but its cost
         }
-        const int rel = u - base;
-        const int rth = rel / it.nt, tile = rel - rth * it.nt;
-        const int head = rth / it.rt, rtile = rth - head * it.rt;
-        const int item0 = u - tile, item1 = item0 + it.nt;
-        const int seg_end = min(u1, item1);
-        const int t0 = it.lo + tile * kKv8Group, t1 = min(r.cap, t0 + (seg_end - u) * kKv8Group);
+    };
+    Piece now;
+    now.u = u0;
+    now.base = base0;
+    now.seq = seq0;
+
+    if (warp == W) {  // ---- the feeding warp: lane w for warp w
+        if (lane < W) {
+            const int hh = lane % hg;
+            int t = 0, n = 0;
+            int id = -1, id_next = -1;  // pages of groups t and t + per_head, and t's scales
+            float ks = 0.0f, vs = 0.0f;
+            now.tb = 0;
+            auto page_of = [&](int at) {
+                const int tok = now.lo + at * kKv8Group;
+                return at < now.tb && tok < now.r.cap ? __ldg(p.c.block_table + (size_t)now.seq * p.c.max_pages + (tok >> plog)) : -1;
+            };
+            auto scales = [&] {
+                if (id >= p.c.n_pages || (id < 0 && t < now.tb && now.lo + t * kKv8Group < now.r.cap)) {
+                    atomicOr(p.s.err, kKv8ErrRange);
+                    id = -1;
+                }
+                ks = id >= 0 ? __ldg(p.c.k_scale + (size_t)id * kvh + now.head + hh) : 0.0f;
+                vs = id >= 0 ? __ldg(p.c.v_scale + (size_t)id * kvh + now.head + hh) : 0.0f;
+            };
+            long long waited = clock64();
+            for (;;) {
+                if (t >= now.tb) {
+                    if (now.u >= u1 || !open(now)) break;
+                    t = now.ta + lane / hg;
+                    id = page_of(t);
+                    id_next = page_of(t + per_head);
+                    scales();
+                    continue;
+                }
+                const int st = n % S::kStages;
+                if (!mbar_test(&s_free[lane][st], ((n / S::kStages) & 1) ^ 1)) {
+                    if (clock64() - waited > kWaitCycles) {
+                        atomicOr(p.s.err, kKv8ErrWait);
+                        break;
+                    }
+                    continue;
+                }
+                s_group[lane][st] = make_float4(ks, vs, __int_as_float(id), 0.0f);
+                mbar_expect_tx(&s_full[lane][st], id >= 0 ? S::kStage : 0);
+                if (id >= 0) {
+                    const int tok = now.lo + t * kKv8Group;
+                    const int row = (int)((((long long)id * kvh + now.head + hh) << plog) + (tok & (p.c.page_size - 1)));
+                    unsigned char* to = ring + (size_t)(lane * S::kStages + st) * S::kStage;
+#pragma unroll
+                    for (int h = 0; h < S::kHalves; ++h) {
+                        tma_load_2d(to + h * S::kBox, &map_k, 128 * h, row, &s_full[lane][st]);
+                        tma_load_2d(to + (S::kHalves + h) * S::kBox, &map_v, 128 * h, row, &s_full[lane][st]);
+                    }
+                }
+                ++n;
+                t += per_head;
+                id = id_next;
+                scales();
+                id_next = page_of(t + per_head);
+                waited = clock64();
+            }
+        }
+        return;
+    }
+
+    auto barrier = [] { asm volatile("bar.sync 1, %0;" ::"n"(S::kThreads) : "memory"); };  // the warps without the feeding one
+    const int hh = warp % hg;  // this warp's head of the item
+    unsigned char* mine_ring = ring + (size_t)warp * S::kStages * S::kStage;
+    // The queries of a piece, a row (of hg * RT) a warp and turn: lane l has dims QE l ..; asked for before anything
+    // waits.
+    constexpr int TURNS = (S::kHeads * RT + W - 1) / W;
+    float qf[QE];
+    auto ask = [&](const Piece& c, int row, float (&f)[QE]) {
+        const int rr = c.rtile * RT + row % RT;
+        if (row < hg * RT && rr < c.r.n * p.gq) {
+            const T* src = static_cast<const T*>(p.q.data) + (size_t)(c.r.row0 + rr / p.gq) * p.q.token_stride +
+                           ((c.head + row / RT) * p.gq + rr % p.gq) * p.q.head_stride + lane * QE;
+#pragma unroll
+            for (int e = 0; e < QE; ++e) f[e] = to_f32(src[e]);
+        }
+    };
+    bool left = now.u < u1 && open(now);
+    if (left) ask(now, warp, qf);
+
+    int n_used = 0;
+    while (left) {
+        const SeqRows& r = now.r;
+        const int head = now.head, rtile = now.rtile;
         const int n_rows = min(RT, r.n * p.gq - rtile * RT);  // rows of this tile
         const int pos_lo = r.start + rtile * RT / p.gq, pos_hi = r.start + (rtile * RT + n_rows - 1) / p.gq;
 
-        // ---- this warp's groups of 16 tokens: t0 + 16 (warp + W i), i < cnt
-        constexpr int STRIDE = W * kKv8Group;
-        const int first = t0 + warp * kKv8Group;
-        const int cnt = first < t1 ? (t1 - first + STRIDE - 1) / STRIDE : 0;
-        const int32_t* table = p.c.block_table + (size_t)seq * p.c.max_pages;
-        // lane l keeps the page of group (i & ~31) + l, looked up when the copies get there, and its scales
-        int ids = -1, ids_before = -1;
-        float kss = 0.0f, vss = 0.0f, kss_before = 0.0f, vss_before = 0.0f;
-        auto look_up = [&](int i) {
-            const int t = first + (i + lane) * STRIDE;
-            ids_before = ids;
-            kss_before = kss;
-            vss_before = vss;
-            ids = -1;
-            if (t < t1) {
-                ids = table[t >> plog];
-                if (ids < 0 || ids >= p.c.n_pages) {
-                    atomicOr(p.s.err, kKv8ErrRange);
-                    ids = -1;
-                }
-            }
-            kss = ids >= 0 ? p.c.k_scale[(size_t)ids * kvh + head] : 0.0f;
-            vss = ids >= 0 ? p.c.v_scale[(size_t)ids * kvh + head] : 0.0f;
-        };
-        auto issue = [&](int i) {  // group i into stage i % kStages
-            if ((i & 31) == 0) look_up(i);
-            const int id = __shfl_sync(0xffffffffu, ids, i & 31);
-            if (lane == 0 && id >= 0) {
-                const int t = first + i * STRIDE, st = i % S::kStages;
-                const int row = (int)((((long long)id * kvh + head) << plog) + (t & (p.c.page_size - 1)));
-                unsigned char* to = mine_ring + st * S::kStage;
-                mbar_expect_tx(&s_full[warp][st], S::kStage);
+        // ---- queries: a warp takes a row, shifts it into fp16's range and rounds it or splits it in two
 #pragma unroll
-                for (int h = 0; h < S::kHalves; ++h) {
-                    tma_load_2d(to + h * S::kBox, &map_k, 128 * h, row, &s_full[warp][st]);
-                    tma_load_2d(to + (S::kHalves + h) * S::kBox, &map_v, 128 * h, row, &s_full[warp][st]);
-                }
-            }
-        };
-        for (int i = 0; i < min(cnt, S::kStages); ++i) issue(i);
-
-        // ---- queries: column g's fragment; dims 64 c + 16 tig + 4 w + {0, 1} and {2, 3} are k-step
-        // 4 c + w's columns 2 tig + {0, 1} and + 8
-        uint32_t bq[KS][2];
-        float rf[2];    // of columns 2 tig, 2 tig + 1: query shift undone, score scale, log2(e)
-        int pos[2];
-        {
-            const int col = TERMS == 2 ? g & 3 : g;
-            const int rr = rtile * RT + col;
-            const bool have = col < n_rows;
-            const T* src = have ? static_cast<const T*>(p.q.data) + (size_t)(r.row0 + rr / p.gq) * p.q.token_stride +
-                                      (head * p.gq + rr % p.gq) * p.q.head_stride
-                                : nullptr;
-            float f[KS][4];
+        for (int turn = 0; turn < TURNS; ++turn) {
+            const int row = warp + turn * W, col = row % RT;
+            if (row >= hg * RT) break;
+            if (turn > 0) ask(now, row, qf);
             float amax = 0.0f;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    f[ks][e] = have ? to_f32(src[(ks >> 2) * 64 + tig * 16 + (ks & 3) * 4 + e]) : 0.0f;
-                    amax = fmaxf(amax, fabsf(f[ks][e]));
-                }
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            const int sh = query_shift(amax);
-            const float up = pow2f(sh);
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    f[ks][e] *= up;
-                    if (TERMS == 2 && g >= 4) f[ks][e] = split_lo(f[ks][e]);
-                }
-                bq[ks][0] = pack_h2(f[ks][0], f[ks][1]);
-                bq[ks][1] = pack_h2(f[ks][2], f[ks][3]);
+            for (int e = 0; e < QE; ++e) {
+                qf[e] = col < n_rows ? qf[e] : 0.0f;
+                amax = fmaxf(amax, fabsf(qf[e]));
             }
-            const float mine = pow2f(-sh) * p.scale_log2;
-            const int c0 = TERMS == 2 ? 2 * (tig & 1) : 2 * tig;
-            rf[0] = __shfl_sync(0xffffffffu, mine, 4 * c0);
-            rf[1] = __shfl_sync(0xffffffffu, mine, 4 * c0 + 4);
+            const int sh = query_shift(warp_max(amax));
+            const float up = pow2f(sh);
+            uint32_t* hi = reinterpret_cast<uint32_t*>(&s_q[row / RT][col][lane * QE]);
+            uint32_t* lo = reinterpret_cast<uint32_t*>(&s_q[row / RT][(col + 4) & 7][lane * QE]);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) pos[h] = c0 + h < n_rows ? r.start + (rtile * RT + c0 + h) / p.gq : -1;
+            for (int e = 0; e < QE; e += 2) {
+                hi[e / 2] = pack_h2(qf[e] * up, qf[e + 1] * up);
+                if (TERMS == 2) lo[e / 2] = pack_h2(split_lo(qf[e] * up), split_lo(qf[e + 1] * up));
+            }
+            if (lane == 0) s_rf[row / RT][col] = pow2f(-sh) * p.scale_log2;
+        }
+        barrier();
+        // column g's fragment: dims 64 c + 16 tig + 4 w + {0, 1} and {2, 3} are k-step 4 c + w's columns
+        // 2 tig + {0, 1} and + 8
+        uint32_t bq[KS][2];
+#pragma unroll
+        for (int c = 0; c < KL; ++c)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const uint4 q = *reinterpret_cast<const uint4*>(&s_q[hh][g][c * 64 + tig * 16 + w * 8]);
+                bq[4 * c + 2 * w][0] = q.x;
+                bq[4 * c + 2 * w][1] = q.y;
+                bq[4 * c + 2 * w + 1][0] = q.z;
+                bq[4 * c + 2 * w + 1][1] = q.w;
+            }
+        float rf[2];  // of columns 2 tig, 2 tig + 1: query shift undone, score scale, log2(e)
+        int pos[2];
+        const int c0 = TERMS == 2 ? 2 * (tig & 1) : 2 * tig;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            rf[h] = s_rf[hh][c0 + h];
+            pos[h] = c0 + h < n_rows ? r.start + (rtile * RT + c0 + h) / p.gq : -1;
         }
 
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
@@ -251,20 +366,15 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
             return HD == 64 ? row * 64 + ((c ^ ((row >> 1) & 3)) << 4) : row * 128 + ((c ^ (row & 7)) << 4);
         };
         const int tok_g = token(g);
-        for (int i = 0; i < cnt; ++i) {
-            const int t = first + i * STRIDE, st = i % S::kStages;
-            // (the copies may already be a batch of 32 look-ups further)
-            const bool older = (i & ~31) != (min(i + S::kStages - 1, cnt - 1) & ~31);
-            const int id = __shfl_sync(0xffffffffu, older ? ids_before : ids, i & 31);
-            const float ks_now = __shfl_sync(0xffffffffu, older ? kss_before : kss, i & 31);
-            const float vs_now = __shfl_sync(0xffffffffu, older ? vss_before : vss, i & 31);
-            const bool bad = id < 0;
+        float unit = 0.0f;  // the value scale that o is in units of
+        for (int tile = now.ta + warp / hg; tile < now.tb; tile += per_head) {
+            const int t = now.lo + tile * kKv8Group, st = n_used % S::kStages;
             const unsigned char* box_k = mine_ring + st * S::kStage;
             const unsigned char* box_v = box_k + S::kHalves * S::kBox;
-            if (!bad) {
-                if (!mbar_wait(&s_full[warp][st], (phases >> st) & 1u, nullptr)) atomicOr(p.s.err, kKv8ErrWait);
-                phases ^= 1u << st;
-            }
+            if (!mbar_wait(&s_full[warp][st], (n_used / S::kStages) & 1, nullptr)) atomicOr(p.s.err, kKv8ErrWait);
+            const float4 group = s_group[warp][st];
+            const float ks_now = group.x, vs_now = group.y;
+            const bool bad = __float_as_int(group.z) < 0;
             // scores of fragment rows g and g + 8, columns 2 tig and 2 tig + 1
             float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sd[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -302,8 +412,9 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
                     }
                 }
             }
+            ++n_used;
             __syncwarp();
-            if (i + S::kStages < cnt) issue(i + S::kStages);
+            if (lane == 0) mbar_arrive(&s_free[warp][st]);
             if (t + kKv8Group > r.cap || bad) {  // what stands behind the last token has no part in the sums
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -342,31 +453,53 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sc[e] = split_lo(sc[e]);
             const uint32_t b0 = transpose8(pack_h2(sc[0], sc[1])), b1 = transpose8(pack_h2(sc[2], sc[3]));
+            // o is kept in units of the largest value scale so far, and at the running maxima: both seldom change, and
+            // then the products go straight into it.  A page of a smaller scale is added in fp32, so no
+            // probability is rounded at another scale than its own.
+            const bool larger = vs_now > unit;
+            if (__any_sync(0xffffffffu, larger || rescale[0] != 1.0f || rescale[1] != 1.0f)) {
+                const float f = larger ? __fdividef(unit, vs_now) : 1.0f;
+                const float f0 = f * rescale[0], f1 = f * rescale[1];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    o[mt][0] *= f0;
+                    o[mt][1] *= f1;
+                    o[mt][2] *= f0;
+                    o[mt][3] *= f1;
+                }
+                unit = larger ? vs_now : unit;
+            }
+            const bool same = vs_now == unit;
+            const float ratio = unit > 0.0f ? __fdividef(vs_now, unit) : 0.0f;
             // values: word c of fragment columns 2 tig, 2 tig + 1 (a, b) and + 8 (cc, d) makes m-tiles 2 c and 2 c + 1,
             // whose rows g and g + 8 are dims 4 c' + {0, 1} and {2, 3} of this lane's piece
+            auto products = [&](auto direct) {
 #pragma unroll
-            for (int c = 0; c < VW; ++c) {
-                const uint32_t ab01 = __byte_perm(vq[0][c], vq[1][c], 0x5140), ab23 = __byte_perm(vq[0][c], vq[1][c], 0x7362);
-                const uint32_t cd01 = __byte_perm(vq[2][c], vq[3][c], 0x5140), cd23 = __byte_perm(vq[2][c], vq[3][c], 0x7362);
+                for (int c = 0; c < VW; ++c) {
+                    const uint32_t ab01 = __byte_perm(vq[0][c], vq[1][c], 0x5140), ab23 = __byte_perm(vq[0][c], vq[1][c], 0x7362);
+                    const uint32_t cd01 = __byte_perm(vq[2][c], vq[3][c], 0x5140), cd23 = __byte_perm(vq[2][c], vq[3][c], 0x7362);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    uint32_t a[4];
-                    codes_to_half<FMT>(e ? ab23 : ab01, a[0], a[1]);
-                    codes_to_half<FMT>(e ? cd23 : cd01, a[2], a[3]);
-                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma_16816(acc, a, b0, b1);
-                    // the page's scale in fp32: no probability is rounded at another scale than its own
-                    float(&om)[4] = o[2 * c + e];
-                    om[0] = fmaf(acc[0], vs_now, om[0] * rescale[0]);
-                    om[1] = fmaf(acc[1], vs_now, om[1] * rescale[1]);
-                    om[2] = fmaf(acc[2], vs_now, om[2] * rescale[0]);
-                    om[3] = fmaf(acc[3], vs_now, om[3] * rescale[1]);
+                    for (int e = 0; e < 2; ++e) {
+                        uint32_t a[4];
+                        codes_to_half<FMT>(e ? ab23 : ab01, a[0], a[1]);
+                        codes_to_half<FMT>(e ? cd23 : cd01, a[2], a[3]);
+                        float(&om)[4] = o[2 * c + e];
+                        if constexpr (decltype(direct)::value) {
+                            mma_16816(om, a, b0, b1);
+                        } else {
+                            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma_16816(acc, a, b0, b1);
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) om[x] = fmaf(acc[x], ratio, om[x]);
+                        }
+                    }
                 }
-            }
+            };
+            if (same) products(std::true_type{});
+            else products(std::false_type{});
         }
 
         // ---- join the warps in warp order
-        __syncthreads();  // every warp's codes are used up
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
@@ -383,95 +516,144 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
             for (int e = 0; e < 4; ++e) {
                 const int c = mt >> 1;
                 const int dim = (VW == 2 ? 8 * g + 4 * c : (c >> 2) * 128 + 16 * g + 4 * (c & 3)) + 2 * (mt & 1) + (e >> 1);
-                s_o[warp][2 * tig + (e & 1)][dim] = o[mt][e];
+                s_o[warp][2 * tig + (e & 1)][dim] = o[mt][e] * unit;
             }
-        __syncthreads();
-        const bool complete = tile == 0 && seg_end == item1;
-        // CTAs that share this row tile: the owner of its first unit to the owner of its last
-        const int cta0 = cut.owner(item0), cta1 = cut.owner(item1 - 1);
-        float* part = p.s.part + (size_t)(2 * blockIdx.x + ((int)blockIdx.x == cta0 ? 1 : 0)) * 8 * PITCH;
-        for (int e = tid; e < n_rows * HD; e += S::kThreads) {
-            const int col = e / HD, d = e - col * HD;
-            float top = -INFINITY, sum = 0.0f, acc = 0.0f;
+        barrier();
+        // the next piece's queries are on their way while this one's results are joined
+        Piece next = now;
+        const bool more_left = next.u < u1 && open(next);
+        if (more_left) ask(next, warp, qf);
+        const bool complete = now.cta0 == now.cta1;
+        constexpr int PART = 64 * PITCH;  // [head of the item][row]
+        float* part = p.s.part + (size_t)(2 * blockIdx.x + ((int)blockIdx.x == now.cta0 ? 1 : 0)) * PART;
+        const int n_out = hg * n_rows;
+        for (int k = warp; k < n_out; k += W) {  // a row's weights: lane i has the i-th warp's of its head
+            const int h = k / n_rows, col = k - h * n_rows;
+            const float wm = lane < per_head ? s_m[h + hg * lane][col] : -INFINITY, wl = lane < per_head ? s_l[h + hg * lane][col] : 0.0f;
+            const float top = warp_max(wm), f = ex2(wm - (top == -INFINITY ? 0.0f : top));
+            float sum = f * wl;
 #pragma unroll
-            for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w][col]);
-            const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float f = ex2(s_m[w][col] - ref);
-                sum = fmaf(f, s_l[w][col], sum);
-                float v = s_o[w][col][d];
-                if (TERMS == 2) v += s_o[w][col + 4][d];
-                acc = fmaf(f, v, acc);
+            for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            if (lane < per_head) s_weight[h + hg * lane][col] = f;
+            if (lane == 0) {
+                s_top[h][col] = top;
+                s_sum[h][col] = sum;
+            }
+        }
+        barrier();
+        auto write = [&](int h, int col, int d, const float4& v, float top, float sum) {
+            const int rr = rtile * RT + col, qh = (head + h) * p.gq + rr % p.gq;
+            const size_t row = (size_t)(r.row0 + rr / p.gq);
+            store_result<T>(p, row, qh, d, v.x, sum);
+            store_result<T>(p, row, qh, d + 1, v.y, sum);
+            store_result<T>(p, row, qh, d + 2, v.z, sum);
+            store_result<T>(p, row, qh, d + 3, v.w, sum);
+            if (d == 0) store_lse(p, row, qh, top, sum);
+        };
+        for (int e = tid; e < n_out * (HD / 4); e += S::kThreads) {
+            const int k = e / (HD / 4), d = (e - k * (HD / 4)) * 4, h = k / n_rows, col = k - h * n_rows;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+            for (int i = 0; i < per_head; ++i) {
+                const int w = h + hg * i;
+                const float f = s_weight[w][col];
+                float4 v = *reinterpret_cast<const float4*>(&s_o[w][col][d]);
+                if (TERMS == 2) {
+                    const float4 lo = *reinterpret_cast<const float4*>(&s_o[w][col + 4][d]);
+                    v = make_float4(v.x + lo.x, v.y + lo.y, v.z + lo.z, v.w + lo.w);
+                }
+                acc = make_float4(fmaf(f, v.x, acc.x), fmaf(f, v.y, acc.y), fmaf(f, v.z, acc.z), fmaf(f, v.w, acc.w));
             }
             if (complete) {
-                const int rr = rtile * RT + col;
-                const size_t row = (size_t)(r.row0 + rr / p.gq);
-                const int qh = head * p.gq + rr % p.gq;
-                store_result<T>(p, row, qh, d, acc, sum);
-                if (d == 0) store_lse(p, row, qh, top, sum);
+                write(h, col, d, acc, s_top[h][col], s_sum[h][col]);
             } else {
-                __stcg(part + col * PITCH + d, acc);
-                if (d == 0) {
-                    __stcg(part + col * PITCH + HD, top);
-                    __stcg(part + col * PITCH + HD + 1, sum);
-                }
+                float* to = part + (h * 8 + col) * PITCH;
+                __stcg(reinterpret_cast<float4*>(to + d), acc);
+                if (d == 0) __stcg(reinterpret_cast<float2*>(to + HD), make_float2(s_top[h][col], s_sum[h][col]));
             }
         }
         if (!complete) {  // the last CTA to arrive joins the parts in CTA order
             __threadfence();
-            __syncthreads();
-            if (tid == 0) s_last = atomicAdd(p.s.ctr + cta0, 1) == cta1 - cta0;
-            __syncthreads();
+            barrier();
+            if (tid == 0) s_last = atomicAdd(p.s.ctr + now.cta0, 1) == now.cta1 - now.cta0;
+            barrier();
             if (s_last) {
                 __threadfence();
-                const int parts = cta1 - cta0 + 1;
-                auto part_of = [&](int k) { return p.s.part + (size_t)(2 * (cta0 + k) + (k == 0 ? 1 : 0)) * 8 * PITCH; };
-                for (int col = warp; col < n_rows; col += W) {
-                    float top = -INFINITY;
-                    for (int k = lane; k < parts; k += 32) top = fmaxf(top, __ldcg(part_of(k) + col * PITCH + HD));
-                    top = warp_max(top);
-                    const float ref = top == -INFINITY ? 0.0f : top;
-                    float sum = 0.0f;
-                    for (int k = lane; k < parts; k += 32)
-                        sum = fmaf(ex2(__ldcg(part_of(k) + col * PITCH + HD) - ref), __ldcg(part_of(k) + col * PITCH + HD + 1), sum);
-#pragma unroll
-                    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-                    if (lane == 0) {
-                        s_top[col] = top;
-                        s_sum[col] = sum;
-                    }
-                }
-                __syncthreads();
-                for (int e = tid; e < n_rows * (HD / 4); e += S::kThreads) {
-                    const int col = e / (HD / 4), d = (e - col * (HD / 4)) * 4;
-                    const float ref = s_top[col] == -INFINITY ? 0.0f : s_top[col];
+                const int parts = now.cta1 - now.cta0 + 1;
+                auto part_of = [&](int k) { return p.s.part + (size_t)(2 * (now.cta0 + k) + (k == 0 ? 1 : 0)) * PART; };
+                // With few rows, groups of threads take every split-th part, so that one trip to L2 (about a
+                // microsecond for what another SM wrote) brings most of them; their sums meet in shared memory.
+                constexpr int B = 8;  // parts in flight
+                const int work = n_out * (HD / 4), split = max(1, min(per_head, S::kThreads / work));
+                const int lanes = split > 1 ? work : S::kThreads, group = split > 1 ? tid / work : 0;
+                auto s_j = reinterpret_cast<float (*)[PITCH]>(s_o);  // [group][row], tops and sums behind the values
+                for (int e = tid - group * lanes; group < split && e < work; e += lanes) {
+                    const int k = e / (HD / 4), d = (e - k * (HD / 4)) * 4, h = k / n_rows, col = k - h * n_rows;
+                    float top = -INFINITY, sum = 0.0f;
                     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-                    for (int k = 0; k < parts; ++k) {
-                        const float* from = part_of(k) + col * PITCH;
-                        const float f = ex2(__ldcg(from + HD) - ref);
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(from + d));
-                        acc.x = fmaf(f, v.x, acc.x);
-                        acc.y = fmaf(f, v.y, acc.y);
-                        acc.z = fmaf(f, v.z, acc.z);
-                        acc.w = fmaf(f, v.w, acc.w);
+                    for (int k0 = group; k0 < parts; k0 += B * split) {
+                        float pm[B], pl[B];
+                        float4 pv[B];
+#pragma unroll
+                        for (int i = 0; i < B; ++i) {
+                            const int at = k0 + i * split;
+                            pm[i] = -INFINITY;
+                            pl[i] = 0.0f;
+                            pv[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (at < parts) {
+                                const float* from = part_of(at) + (h * 8 + col) * PITCH;
+                                const float2 ml = __ldcg(reinterpret_cast<const float2*>(from + HD));
+                                pv[i] = __ldcg(reinterpret_cast<const float4*>(from + d));
+                                pm[i] = ml.x;
+                                pl[i] = ml.y;
+                            }
+                        }
+                        const float before = top;
+#pragma unroll
+                        for (int i = 0; i < B; ++i) top = fmaxf(top, pm[i]);
+                        const float ref = top == -INFINITY ? 0.0f : top;
+                        const float f0 = ex2(before - ref);
+                        sum *= f0;
+                        acc = make_float4(acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0);
+#pragma unroll
+                        for (int i = 0; i < B; ++i) {
+                            const float f = ex2(pm[i] - ref);
+                            sum = fmaf(f, pl[i], sum);
+                            acc = make_float4(fmaf(f, pv[i].x, acc.x), fmaf(f, pv[i].y, acc.y), fmaf(f, pv[i].z, acc.z), fmaf(f, pv[i].w, acc.w));
+                        }
                     }
-                    const int rr = rtile * RT + col;
-                    const size_t row = (size_t)(r.row0 + rr / p.gq);
-                    const int qh = head * p.gq + rr % p.gq;
-                    store_result<T>(p, row, qh, d, acc.x, s_sum[col]);
-                    store_result<T>(p, row, qh, d + 1, acc.y, s_sum[col]);
-                    store_result<T>(p, row, qh, d + 2, acc.z, s_sum[col]);
-                    store_result<T>(p, row, qh, d + 3, acc.w, s_sum[col]);
-                    if (d == 0) store_lse(p, row, qh, s_top[col], s_sum[col]);
+                    if (split == 1) {
+                        write(h, col, d, acc, top, sum);
+                    } else {
+                        *reinterpret_cast<float4*>(&s_j[group * n_out + k][d]) = acc;
+                        if (d == 0) *reinterpret_cast<float2*>(&s_j[group * n_out + k][HD]) = make_float2(top, sum);
+                    }
                 }
-                if (tid == 0) p.s.ctr[cta0] = 0;  // ready for the next call
+                if (split > 1) {
+                    barrier();
+                    for (int e = tid; e < work; e += S::kThreads) {
+                        const int k = e / (HD / 4), d = (e - k * (HD / 4)) * 4, h = k / n_rows, col = k - h * n_rows;
+                        float top = -INFINITY, sum = 0.0f;
+                        float4 out = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        for (int i = 0; i < split; ++i) top = fmaxf(top, s_j[i * n_out + k][HD]);
+                        const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll 4
+                        for (int i = 0; i < split; ++i) {
+                            const float2 ml = *reinterpret_cast<const float2*>(&s_j[i * n_out + k][HD]);
+                            const float4 v = *reinterpret_cast<const float4*>(&s_j[i * n_out + k][d]);
+                            const float f = ex2(ml.x - ref);
+                            sum = fmaf(f, ml.y, sum);
+                            out = make_float4(fmaf(f, v.x, out.x), fmaf(f, v.y, out.y), fmaf(f, v.z, out.z), fmaf(f, v.w, out.w));
+                        }
+                        write(h, col, d, out, top, sum);
+                    }
+                }
+                if (tid == 0) p.s.ctr[now.cta0] = 0;  // ready for the next call
             }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring is the copies' again
-        __syncthreads();
-        u = seg_end;
+        // (the next piece's queries pass a barrier before anything of this one's is overwritten)
+        now = next;
+        left = more_left;
     }
 }
 
@@ -493,7 +675,7 @@ int make_map(CUtensorMap* map, const void* codes, const iam_kv8_cache& c) {
 
 template <class T, int FMT, int HD>
 int launch(const Kv8Attn& a, cudaStream_t s) {
-    constexpr size_t smem = Shape<HD>::kRing + 1024;
+    constexpr size_t smem = Shape<HD>::kSmem;
     auto kern = kv8_decode_kernel<T, FMT, HD, sizeof(T) == 4 ? 2 : 1>;
     static std::atomic<unsigned long long> done{0};
     IAM_CUDA_TRY(once_per_device(done, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }));
@@ -501,7 +683,10 @@ int launch(const Kv8Attn& a, cudaStream_t s) {
     int rc = make_map<HD>(&mk, a.c.k, a.c);
     if (rc == IAM_OK) rc = make_map<HD>(&mv, a.c.v, a.c);
     if (rc) return rc;
-    kern<<<a.sms, Shape<HD>::kThreads, smem, s>>>(a, mk, mv);
+    // KV heads of an item: more than one only where (sequence, head) pairs outnumber the SMs
+    int hg = 1;
+    while (hg < Shape<HD>::kHeads && a.c.n_kv_heads % (2 * hg) == 0 && (long long)a.c.n_seqs * (a.c.n_kv_heads / hg) > a.sms) hg *= 2;
+    kern<<<a.sms, Shape<HD>::kThreads + 32, smem, s>>>(a, hg, mk, mv);
     IAM_CUDA_TRY(cudaGetLastError());
     return IAM_OK;
 }
@@ -518,7 +703,7 @@ int launch_dim(const Kv8Attn& a, cudaStream_t s) {
 }  // namespace
 
 int kv8_max_ctas(int sms) { return 4 * sms; }
-size_t kv8_decode_part_floats(int head_dim, int sms) { return (size_t)2 * sms * 8 * (head_dim + 4); }
+size_t kv8_decode_part_floats(int head_dim, int sms) { return (size_t)2 * sms * 64 * (head_dim + 4); }
 
 int kv8_decode_launch(const Kv8Attn& a, int dtype, cudaStream_t s) {
     return with_dtype(dtype, [&](auto t) {
