@@ -70,6 +70,14 @@ IAM_DEV float warp_max(float v) {
     return v;
 }
 
+// Counts one arrival, with what the CTA's threads wrote before their last barrier, and returns the number before it;
+// what earlier arrivals brought is visible to the CTA behind its next barrier.
+IAM_DEV int arrive(int* ctr) {
+    int before;
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(__cvta_generic_to_global(ctr)) : "memory");
+    return before;
+}
+
 constexpr float kLn2 = 0.69314718055994530942f;
 
 // A row's result from its running maximum (log2 domain), sum and value sums.

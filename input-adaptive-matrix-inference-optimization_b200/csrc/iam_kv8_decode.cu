@@ -19,19 +19,19 @@ namespace {
 constexpr int kMinGroups = 8;  // groups of tokens of a CTA at least, where a context is shared
 constexpr int kItemCost = 24;  // what opening and joining a piece of a context costs, in groups
 
-// Warps of a CTA (one CTA an SM; one warp more feeds them) and groups of 16 tokens in each warp's ring: 128 KB of
-// codes on their way.
+// Warps of a CTA (one CTA an SM; as many as have the registers they need) and groups of 16 tokens in each warp's
+// ring: 128 to 144 KB of codes on their way.
 template <int HD>
 struct Shape {
-    static constexpr int kWarps = HD == 256 ? 8 : 16;
+    static constexpr int kWarps = HD == 256 ? 8 : HD == 128 ? 12 : 16;
     static constexpr int kThreads = 32 * kWarps;
     static constexpr int kHalves = HD == 256 ? 2 : 1;          // 128-byte columns of a row
     static constexpr int kBox = kKv8Group * HD / kHalves;      // bytes of one copy
     static constexpr int kStage = 2 * kHalves * kBox;          // a group's keys and values
-    static constexpr int kStages = 128 * 1024 / (kWarps * kStage);
+    static constexpr int kStages = HD == 256 ? 2 : HD == 128 ? 3 : 4;
     static constexpr int kRing = kWarps * kStages * kStage;
     static constexpr int kPitch = HD + 4;
-    static constexpr int kHeads = HD == 256 ? 4 : 8;            // heads of an item at most
+    static constexpr int kHeads = HD == 64 ? 8 : 4;             // heads of an item at most
     static constexpr int kSmem = kRing + kWarps * 8 * kPitch * 4 + 1024;
 };
 
@@ -82,21 +82,22 @@ IAM_DEV uint32_t transpose8(uint32_t v) {
 
 // T: query and output type; TERMS 2 (fp32): columns 0..3 of the tile hold the rows' high fp16 terms and
 // 4..7 the low ones (and so for the probabilities), which carries 22 bits of both through fp16 products.
-// Each warp has a ring of its own in shared memory, and lane w of the feeding warp keeps warp w's full: it has TMA
-// fetch a group's keys and values (16 rows each, swizzled so that the reads below meet no bank twice) as soon as
-// the warp has taken an earlier group out of that place, into the next piece of context already; the warps
-// wait for one another only to join a piece's results.  The fragments' rows are tokens in the order
-// 0 4 2 6 5 1 7 3 for the same reason: eight lanes then read eight different 16-byte columns both as keys (two
-// tokens, four columns) and as values (four tokens, two columns).
+// Each warp streams its own groups of tokens through its own ring in shared memory: TMA fetches a group's keys and
+// values (16 rows each, swizzled so that the reads below meet no bank twice) as soon as the warp has taken an
+// earlier group out of that place, into the next piece of context already; the warps wait for one another only
+// to join a piece's results.  (One feeding warp for all of them was slower: its lanes share the wait for each
+// look-up.)  The fragments' rows are tokens in the order 0 4 2 6 5 1 7 3 for the same reason: eight lanes then
+// read eight different 16-byte columns both as keys (two tokens, four columns) and as values (four tokens, two
+// columns).
 template <class T, int FMT, int HD, int TERMS>
-__global__ void __launch_bounds__(Shape<HD>::kThreads + 32, 1)
+__global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
     kv8_decode_kernel(const Kv8Attn p, int hg, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
     using S = Shape<HD>;
     constexpr int RT = 8 / TERMS, W = S::kWarps;
     constexpr int KS = HD / 16, KL = HD / 64, VW = HD / 32, MT = HD / 16;
     constexpr int PITCH = S::kPitch, QE = HD / 32;
     extern __shared__ unsigned char s_raw[];
-    __shared__ __align__(8) uint64_t s_full[W][S::kStages], s_free[W][S::kStages];
+    __shared__ __align__(8) uint64_t s_full[W][S::kStages];
     __shared__ float4 s_group[W][S::kStages];  // key scale, value scale, page (as bits) of the group in a place
     __shared__ __align__(16) __half s_q[S::kHeads][8][HD + 8];  // [head of the item][column]
     __shared__ float s_rf[S::kHeads][8];
@@ -108,18 +109,15 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads + 32, 1)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tig = lane & 3;
     const int plog = 31 - __clz(p.c.page_size), kvh = p.c.n_kv_heads;
     const int per_head = W / hg;  // warps that share a head
-    if (tid < W) {
-        for (int i = 0; i < S::kStages; ++i) {
-            mbar_init(&s_full[tid][i], 1);
-            mbar_init(&s_free[tid][i], 1);
-        }
+    if (lane == 0) {
+        for (int i = 0; i < S::kStages; ++i) mbar_init(&s_full[warp][i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (tid == W) {
+    if (tid == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
     }
-    __syncthreads();
+    __syncwarp();
 
     // ---- this CTA's run (every warp finds it by itself)
     long long n_items = 0, n_groups = 0;
@@ -170,8 +168,8 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads + 32, 1)
         if (i0 + 32 >= p.c.n_seqs) return;  // (few: more CTAs than shares)
     }
 
-    // A piece of an item: groups [ta, tb) of it, shared by CTAs cta0 .. cta1.  The feeding lanes walk the pieces
-    // ahead of the warps.
+    // A piece of an item: groups [ta, tb) of it, shared by CTAs cta0 .. cta1.  One state walks the pieces for the
+    // copies, another one behind it for the sums.
     struct Piece {
         int u, base, seq;  // place on the line, units (or CTAs) before the sequence
         SeqRows r;
@@ -220,67 +218,6 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads + 32, 1)
     now.base = base0;
     now.seq = seq0;
 
-    if (warp == W) {  // ---- the feeding warp: lane w for warp w
-        if (lane < W) {
-            const int hh = lane % hg;
-            int t = 0, n = 0;
-            int id = -1, id_next = -1;  // pages of groups t and t + per_head, and t's scales
-            float ks = 0.0f, vs = 0.0f;
-            now.tb = 0;
-            auto page_of = [&](int at) {
-                const int tok = now.lo + at * kKv8Group;
-                return at < now.tb && tok < now.r.cap ? __ldg(p.c.block_table + (size_t)now.seq * p.c.max_pages + (tok >> plog)) : -1;
-            };
-            auto scales = [&] {
-                if (id >= p.c.n_pages || (id < 0 && t < now.tb && now.lo + t * kKv8Group < now.r.cap)) {
-                    atomicOr(p.s.err, kKv8ErrRange);
-                    id = -1;
-                }
-                ks = id >= 0 ? __ldg(p.c.k_scale + (size_t)id * kvh + now.head + hh) : 0.0f;
-                vs = id >= 0 ? __ldg(p.c.v_scale + (size_t)id * kvh + now.head + hh) : 0.0f;
-            };
-            long long waited = clock64();
-            for (;;) {
-                if (t >= now.tb) {
-                    if (now.u >= u1 || !open(now)) break;
-                    t = now.ta + lane / hg;
-                    id = page_of(t);
-                    id_next = page_of(t + per_head);
-                    scales();
-                    continue;
-                }
-                const int st = n % S::kStages;
-                if (!mbar_test(&s_free[lane][st], ((n / S::kStages) & 1) ^ 1)) {
-                    if (clock64() - waited > kWaitCycles) {
-                        atomicOr(p.s.err, kKv8ErrWait);
-                        break;
-                    }
-                    continue;
-                }
-                s_group[lane][st] = make_float4(ks, vs, __int_as_float(id), 0.0f);
-                mbar_expect_tx(&s_full[lane][st], id >= 0 ? S::kStage : 0);
-                if (id >= 0) {
-                    const int tok = now.lo + t * kKv8Group;
-                    const int row = (int)((((long long)id * kvh + now.head + hh) << plog) + (tok & (p.c.page_size - 1)));
-                    unsigned char* to = ring + (size_t)(lane * S::kStages + st) * S::kStage;
-#pragma unroll
-                    for (int h = 0; h < S::kHalves; ++h) {
-                        tma_load_2d(to + h * S::kBox, &map_k, 128 * h, row, &s_full[lane][st]);
-                        tma_load_2d(to + (S::kHalves + h) * S::kBox, &map_v, 128 * h, row, &s_full[lane][st]);
-                    }
-                }
-                ++n;
-                t += per_head;
-                id = id_next;
-                scales();
-                id_next = page_of(t + per_head);
-                waited = clock64();
-            }
-        }
-        return;
-    }
-
-    auto barrier = [] { asm volatile("bar.sync 1, %0;" ::"n"(S::kThreads) : "memory"); };  // the warps without the feeding one
     const int hh = warp % hg;  // this warp's head of the item
     unsigned char* mine_ring = ring + (size_t)warp * S::kStages * S::kStage;
     // The queries of a piece, a row (of hg * RT) a warp and turn: lane l has dims QE l ..; asked for before anything
@@ -296,8 +233,55 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads + 32, 1)
             for (int e = 0; e < QE; ++e) f[e] = to_f32(src[e]);
         }
     };
+    // The stream of the warp's groups, kStages ahead of their use and into the next pieces.
     bool left = now.u < u1 && open(now);
+    Piece ahead = now;
+    int t_ahead = now.ta + warp / hg, n_issued = 0, batch = 32;
+    bool more = left;
+    int ids = -1;  // lane l: page and scales of group t_ahead + per_head l, as of the last look-up
+    float kss = 0.0f, vss = 0.0f;
+    auto issue = [&] {
+        while (more && t_ahead >= ahead.tb) {
+            more = ahead.u < u1 && open(ahead);
+            if (more) t_ahead = ahead.ta + warp / hg;
+            batch = 32;
+        }
+        if (!more) return;
+        if (batch == 32) {
+            const int t = t_ahead + per_head * lane;
+            ids = -1;
+            if (t < ahead.tb && ahead.lo + t * kKv8Group < ahead.r.cap) {
+                ids = __ldg(p.c.block_table + (size_t)ahead.seq * p.c.max_pages + ((ahead.lo + t * kKv8Group) >> plog));
+                if (ids < 0 || ids >= p.c.n_pages) {
+                    atomicOr(p.s.err, kKv8ErrRange);
+                    ids = -1;
+                }
+            }
+            kss = ids >= 0 ? __ldg(p.c.k_scale + (size_t)ids * kvh + ahead.head + hh) : 0.0f;
+            vss = ids >= 0 ? __ldg(p.c.v_scale + (size_t)ids * kvh + ahead.head + hh) : 0.0f;
+            batch = 0;
+        }
+        if (lane == batch) {  // the lane that looked it up
+            const int st = n_issued % S::kStages;
+            mbar_expect_tx(&s_full[warp][st], ids >= 0 ? S::kStage : 0);
+            if (ids >= 0) {
+                const int tok = ahead.lo + t_ahead * kKv8Group;
+                const int row = (int)((((long long)ids * kvh + ahead.head + hh) << plog) + (tok & (p.c.page_size - 1)));
+                unsigned char* to = mine_ring + st * S::kStage;
+#pragma unroll
+                for (int h = 0; h < S::kHalves; ++h) {
+                    tma_load_2d(to + h * S::kBox, &map_k, 128 * h, row, &s_full[warp][st]);
+                    tma_load_2d(to + (S::kHalves + h) * S::kBox, &map_v, 128 * h, row, &s_full[warp][st]);
+                }
+            }
+            s_group[warp][st] = make_float4(kss, vss, __int_as_float(ids), 0.0f);  // (the copies do not wait for the scales)
+        }
+        ++n_issued;
+        ++batch;
+        t_ahead += per_head;
+    };
     if (left) ask(now, warp, qf);
+    for (int i = 0; i < S::kStages; ++i) issue();
 
     int n_used = 0;
     while (left) {
@@ -329,7 +313,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads + 32, 1)
             }
             if (lane == 0) s_rf[row / RT][col] = pow2f(-sh) * p.scale_log2;
         }
-        barrier();
+        __syncthreads();
         // column g's fragment: dims 64 c + 16 tig + 4 w + {0, 1} and {2, 3} are k-step 4 c + w's columns
         // 2 tig + {0, 1} and + 8
         uint32_t bq[KS][2];
@@ -414,7 +398,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads + 32, 1)
             }
             ++n_used;
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s_free[warp][st]);
+            issue();
             if (t + kKv8Group > r.cap || bad) {  // what stands behind the last token has no part in the sums
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -518,7 +502,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads + 32, 1)
                 const int dim = (VW == 2 ? 8 * g + 4 * c : (c >> 2) * 128 + 16 * g + 4 * (c & 3)) + 2 * (mt & 1) + (e >> 1);
                 s_o[warp][2 * tig + (e & 1)][dim] = o[mt][e] * unit;
             }
-        barrier();
+        __syncthreads();
         // the next piece's queries are on their way while this one's results are joined
         Piece next = now;
         const bool more_left = next.u < u1 && open(next);
@@ -540,7 +524,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads + 32, 1)
                 s_sum[h][col] = sum;
             }
         }
-        barrier();
+        __syncthreads();
         auto write = [&](int h, int col, int d, const float4& v, float top, float sum) {
             const int rr = rtile * RT + col, qh = (head + h) * p.gq + rr % p.gq;
             const size_t row = (size_t)(r.row0 + rr / p.gq);
@@ -573,12 +557,10 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads + 32, 1)
             }
         }
         if (!complete) {  // the last CTA to arrive joins the parts in CTA order
-            __threadfence();
-            barrier();
-            if (tid == 0) s_last = atomicAdd(p.s.ctr + now.cta0, 1) == now.cta1 - now.cta0;
-            barrier();
+            __syncthreads();
+            if (tid == 0) s_last = arrive(p.s.ctr + now.cta0) == now.cta1 - now.cta0;
+            __syncthreads();
             if (s_last) {
-                __threadfence();
                 const int parts = now.cta1 - now.cta0 + 1;
                 auto part_of = [&](int k) { return p.s.part + (size_t)(2 * (now.cta0 + k) + (k == 0 ? 1 : 0)) * PART; };
                 // With few rows, groups of threads take every split-th part, so that one trip to L2 (about a
@@ -630,7 +612,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads + 32, 1)
                     }
                 }
                 if (split > 1) {
-                    barrier();
+                    __syncthreads();
                     for (int e = tid; e < work; e += S::kThreads) {
                         const int k = e / (HD / 4), d = (e - k * (HD / 4)) * 4, h = k / n_rows, col = k - h * n_rows;
                         float top = -INFINITY, sum = 0.0f;
@@ -686,7 +668,7 @@ int launch(const Kv8Attn& a, cudaStream_t s) {
     // KV heads of an item: more than one only where (sequence, head) pairs outnumber the SMs
     int hg = 1;
     while (hg < Shape<HD>::kHeads && a.c.n_kv_heads % (2 * hg) == 0 && (long long)a.c.n_seqs * (a.c.n_kv_heads / hg) > a.sms) hg *= 2;
-    kern<<<a.sms, Shape<HD>::kThreads + 32, smem, s>>>(a, hg, mk, mv);
+    kern<<<a.sms, Shape<HD>::kThreads, smem, s>>>(a, hg, mk, mv);
     IAM_CUDA_TRY(cudaGetLastError());
     return IAM_OK;
 }

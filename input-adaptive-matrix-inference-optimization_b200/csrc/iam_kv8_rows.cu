@@ -396,12 +396,10 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(Kv8Attn p) {
             }
         }
         if (!complete) {  // the last CTA to arrive joins the parts in CTA order
-            __threadfence();
             __syncthreads();
-            if (tid == 0) s_last = atomicAdd(p.s.ctr + cta0, 1) == cta1 - cta0;
+            if (tid == 0) s_last = arrive(p.s.ctr + cta0) == cta1 - cta0;
             __syncthreads();
             if (s_last) {
-                __threadfence();
                 const int parts = cta1 - cta0 + 1;
                 auto part_of = [&](int k) { return p.s.part + (size_t)(2 * (cta0 + k) + (k == 0 ? 1 : 0)) * kRows * PITCH; };
                 for (int row = warp; row < it.n_rows; row += kThreads / 32) {
