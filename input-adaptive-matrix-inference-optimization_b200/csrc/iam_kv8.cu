@@ -221,7 +221,7 @@ extern "C" int iam_kv8_create(iam_kv8_t* out, int n_heads, int n_kv_heads, int h
     h->n_kv_heads = n_kv_heads;
     h->head_dim = head_dim;
     h->s.max_ctas = kv8_max_ctas(sms);
-    h->s.part_floats = std::max(kv8_decode_part_floats(head_dim, sms), kv8_rows_part_floats(head_dim, sms));
+    h->s.part_floats = std::max(std::max(kv8_decode_part_floats(head_dim, sms), kv8_rows_part_floats(head_dim, sms)), kv8_prompt_part_floats(head_dim, sms));
     cudaError_t e = cudaMalloc(&h->s.part, h->s.part_floats * sizeof(float));
     if (e == cudaSuccess) e = cudaMalloc(&h->s.ctr, h->s.max_ctas * sizeof(int));
     if (e == cudaSuccess) e = cudaMemset(h->s.ctr, 0, h->s.max_ctas * sizeof(int));
@@ -333,5 +333,9 @@ extern "C" int iam_kv8_attention(iam_kv8_t h, const iam_kv8_cache* cache, int dt
     DeviceGuard g(h->device);
     IAM_CUDA_TRY(g.err);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return rows <= (dtype == IAM_F32 ? 4 : 8) ? kv8_decode_launch(a, dtype, s) : kv8_rows_launch(a, dtype, s);
+    if ((long long)n_rows * a.gq / 64 + cache->n_seqs > kKv8MaxItems)
+        return fail(IAM_ERR_ARG, "kv8: more query rows than one call takes (65536 tiles of 64)");
+    if (rows <= (dtype == IAM_F32 ? 4 : 8)) return kv8_decode_launch(a, dtype, s);
+    if (dtype != IAM_F32 && h->head_dim <= 128 && rows > 64) return kv8_prompt_launch(a, dtype, s);
+    return kv8_rows_launch(a, dtype, s);
 }

@@ -39,8 +39,10 @@ struct Kv8Attn {
 
 int kv8_decode_launch(const Kv8Attn& a, int dtype, cudaStream_t s);
 int kv8_rows_launch(const Kv8Attn& a, int dtype, cudaStream_t s);
+int kv8_prompt_launch(const Kv8Attn& a, int dtype, cudaStream_t s);  // 16-bit queries, head_dim 64 or 128
 size_t kv8_decode_part_floats(int head_dim, int sms);
 size_t kv8_rows_part_floats(int head_dim, int sms);
+size_t kv8_prompt_part_floats(int head_dim, int sms);
 int kv8_max_ctas(int sms);
 size_t kv8_plan_words();
 

@@ -3,7 +3,7 @@
 #include <algorithm>
 #include <atomic>
 
-#include "iam_kv8.cuh"
+#include "iam_kv8_plan.cuh"
 
 namespace iam {
 namespace {
@@ -12,94 +12,6 @@ constexpr int kRows = 64;       // query rows of a tile: 16 for each warp
 constexpr int kThreads = 128;
 constexpr int kTile = 64;       // tokens of a work unit
 constexpr int kPerSm = 3;       // CTAs per SM at most (scratch)
-constexpr int kPlanThreads = 1024;
-
-// Words of the schedule: the number of row tiles; then, of each, its sequence, its number within the
-// sequence, and the units of tokens before it (one more entry: all units).
-struct Plan {
-    int* words;
-    IAM_DEV int& items() const { return words[0]; }
-    IAM_DEV int* seq() const { return words + 1; }
-    IAM_DEV int* rtile() const { return words + 1 + kKv8MaxItems; }
-    IAM_DEV int* unit() const { return words + 1 + 2 * kKv8MaxItems; }
-};
-
-struct Item {
-    int lo, nt, pos_lo, pos_hi, n_rows;  // first token read (a multiple of kTile), units, first and last position
-};
-
-IAM_DEV Item item_of(const Kv8Attn& p, const SeqRows& r, int rtile) {
-    Item it;
-    it.n_rows = min(kRows, r.n * p.gq - rtile * kRows);
-    it.pos_lo = r.start + rtile * kRows / p.gq;
-    it.pos_hi = r.start + (rtile * kRows + it.n_rows - 1) / p.gq;
-    it.lo = p.window > 0 ? max(0, it.pos_lo - p.window + 1) & ~(kTile - 1) : 0;
-    const int hi = min(it.pos_hi + 1, r.cap);
-    it.nt = max(1, (hi - it.lo + kTile - 1) / kTile);
-    return it;
-}
-
-IAM_DEV int block_scan(int v, int* s_warp, int& total) {  // exclusive
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int sum = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += up;
-    }
-    __syncthreads();  // (s_warp of an earlier call is consumed)
-    if (lane == 31) s_warp[warp] = sum;
-    __syncthreads();
-    if (warp == 0) {
-        int w = s_warp[lane];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += up;
-        }
-        s_warp[lane] = w;
-    }
-    __syncthreads();
-    total = s_warp[kPlanThreads / 32 - 1];
-    return sum - v + (warp ? s_warp[warp - 1] : 0);
-}
-
-// The row tiles of the call in order, and how many units of tokens stand before each.
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(Kv8Attn p) {
-    __shared__ int s_warp[32];
-    const Plan plan{p.s.plan};
-    const int tid = threadIdx.x;
-    int items = 0, total;
-    for (int i0 = 0; i0 < p.c.n_seqs; i0 += kPlanThreads) {
-        const int i = i0 + tid;
-        int n = 0;
-        if (i < p.c.n_seqs) n = (seq_rows(p.c, p.cu, p.lens, p.n_rows, i, p.s.err).n * p.gq + kRows - 1) / kRows;
-        const int at = items + block_scan(n, s_warp, total);
-        for (int k = 0; k < n && at + k < kKv8MaxItems; ++k) {
-            plan.seq()[at + k] = i;
-            plan.rtile()[at + k] = k;
-        }
-        items = min(items + total, kKv8MaxItems);  // (more only when the row offsets do not ascend)
-    }
-    __syncthreads();
-    int units = 0;
-    for (int i0 = 0; i0 < items; i0 += kPlanThreads) {
-        const int i = i0 + tid;
-        int n = 0;
-        if (i < items) {
-            const int seq = plan.seq()[i];
-            n = item_of(p, seq_rows(p.c, p.cu, p.lens, p.n_rows, seq, nullptr), plan.rtile()[i]).nt;
-        }
-        const int at = units + block_scan(n, s_warp, total);
-        if (i < items) plan.unit()[i] = at;
-        units += total;
-    }
-    if (tid == 0) {
-        plan.unit()[items] = units;
-        plan.items() = items;
-    }
-}
-
 // Row tile (16 rows a warp) times tokens: scores with the queries as A and the tokens as B of m16n8k16, the
 // probabilities (fp16, one or two terms) from the accumulators' own registers as A and the values as B.
 // Codes arrive by cp.async one tile ahead and become fp16 in shared memory once per tile for all warps.
@@ -130,20 +42,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(Kv8Attn p) {
     const long long ctas = min((long long)gridDim.x, total);
     if (blockIdx.x >= ctas) return;
     const long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
-    int item;
-    {   // the last row tile whose first unit is at most u0's: 32 probes a round
-        const int want = (int)(u0 % per_head);
-        int lo = 0, hi = items;  // unit[lo] <= want < unit[hi]
-        while (hi - lo > 1) {
-            const int step = (hi - lo + 31) / 32;
-            const int at = min(lo + lane * step, hi);
-            const unsigned le = __ballot_sync(0xffffffffu, at < hi && plan.unit()[at] <= want);
-            const int last = 31 - __clz(le);  // lane 0 always holds
-            hi = min(hi, lo + (last + 1) * step);
-            lo = lo + last * step;
-        }
-        item = lo;
-    }
+    int item = find_item(plan, items, (int)(u0 % per_head));
     int head = (int)(u0 / per_head);
 
     long long u = u0;
@@ -151,7 +50,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(Kv8Attn p) {
         const long long item0 = (long long)head * per_head + plan.unit()[item], item1 = (long long)head * per_head + plan.unit()[item + 1];
         const int seq = plan.seq()[item], rtile = plan.rtile()[item];
         const SeqRows r = seq_rows(p.c, p.cu, p.lens, p.n_rows, seq, nullptr);
-        const Item it = item_of(p, r, rtile);
+        const RowItem it = item_of<kRows, kTile>(p, r, rtile);
         const int tile = (int)(u - item0);
         const long long seg_end = min(u1, item1);
         const int n_tiles = (int)(seg_end - u);
@@ -450,7 +349,7 @@ int launch(const Kv8Attn& a, cudaStream_t s) {
         IAM_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, kThreads, smem));
         resident.store(n, std::memory_order_relaxed);
     }
-    plan_kernel<<<1, kPlanThreads, 0, s>>>(a);
+    plan_kernel<kRows, kTile><<<1, kPlanThreads, 0, s>>>(a);
     IAM_CUDA_TRY(cudaGetLastError());
     kern<<<std::min(kPerSm, n) * a.sms, kThreads, smem, s>>>(a);
     IAM_CUDA_TRY(cudaGetLastError());
@@ -472,8 +371,6 @@ size_t kv8_plan_words() { return 2 + 3 * (size_t)kKv8MaxItems; }
 size_t kv8_rows_part_floats(int head_dim, int sms) { return (size_t)2 * kPerSm * sms * kRows * (head_dim + 4); }
 
 int kv8_rows_launch(const Kv8Attn& a, int dtype, cudaStream_t s) {
-    if ((long long)a.n_rows * a.gq / kRows + a.c.n_seqs > kKv8MaxItems)
-        return fail(IAM_ERR_ARG, "kv8: more query rows than one call takes (65536 tiles of 64)");
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         return a.c.format == IAM_KV8_INT8 ? launch_dim<T, IAM_KV8_INT8>(a, s) : launch_dim<T, IAM_KV8_E4M3>(a, s);
