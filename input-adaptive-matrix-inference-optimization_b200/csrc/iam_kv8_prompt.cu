@@ -1,18 +1,21 @@
 // iam_kv8_prompt.cu -- attention of prompts over the 8-bit paged cache on the tcgen05 tensor cores (fp16 and bf16
 // queries, head_dim 64 and 128).
 //
-// A CTA holds two tiles of 128 query rows and walks the tokens 128 at a time.  Scores S = Q K^T and values O += P V are
-// tcgen05.mma (fp16 products, fp32 sums in tensor memory: S of both tiles, with P over it as the left operand, and O
-// of both: 512 columns).  The codes become fp16 in shared memory once for both row tiles.  By warp:
+// A CTA holds two tiles of 128 query rows and walks the tokens 64 at a time.  Scores S = Q K^T and values O += P V are
+// tcgen05.mma (fp16 products, fp32 sums in tensor memory: for each row tile two S, with P over it as the left
+// operand, and O: 512 columns).  S of the next tokens is computed while the softmax works on this one's, so the
+// softmax, which bounds the kernel, never waits for it (one S of 128 tokens, which it waits for, took 1.2 times as
+// long).  The codes become fp16 in shared memory once for both row tiles.  By warp:
 //   0..3, 4..7   softmax of row tile 0, 1: a thread owns a row, so maxima and sums need no exchange
 //   8..11        codes to fp16: keys as they lie, values turned so that a dim's tokens are adjacent (both operands
 //                are then K-major with the 128-byte swizzle)
 //   12           the MMAs, issued by one thread: while one row tile's probabilities are made, the other's products run
 //   13           the copies (TMA, 16 rows a box, so any page size)
-// A tile of 128 x 128 x 128 costs the tensor cores 512 cycles for S and as many for P V, and its 16384 powers cost the
-// special-function units 1024: the two are level, and neither can wait for the other, hence two row tiles.
+// 128 x 128 rows and tokens cost the tensor cores 512 cycles for S and as many for P V (head_dim 128), and their 16384
+// powers cost the special-function units 1024: the two are level, and neither can wait for the other.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "iam_kv8_plan.cuh"
 #include "iam_tc.cuh"
@@ -22,11 +25,11 @@ namespace {
 
 constexpr int kQ = 128;            // rows of a tile: the MMA's M
 constexpr int kRows = 2 * kQ;
-constexpr int kTile = 128;         // tokens of a unit
+constexpr int kTile = 64;          // tokens of a unit
 constexpr int kGroups = kTile / kKv8Group;
-constexpr int kThreads = 14 * 32;
-constexpr int kInfo = 4;           // tiles whose scales are kept: the softmax may be two behind the copies
-constexpr float kLift = 128.0f;    // probabilities (at most 2^kLag) are lifted before they are rounded to fp16
+constexpr int kThreads = 16 * 32;  // (warps 14 and 15 only complete the last four)
+constexpr int kInfo = 8;           // tiles whose scales are kept: the softmax may be four behind the copies
+constexpr int kLiftLog = 7;        // probabilities (at most 2^kLag) are lifted by 2^kLiftLog before they are rounded to fp16
 constexpr float kLag = 8.0f;       // a row's reference is raised when its maximum outgrows it by more than this (log2)
 
 template <int HD>
@@ -36,8 +39,8 @@ struct Smem {
     static constexpr int kHalf = kTile * HD * 2;        // the same in fp16
     static constexpr int q = 0;                         // [2] row tiles
     static constexpr int k16 = 2 * kQBytes;
-    static constexpr int v16 = k16 + kHalf;
-    static constexpr int raw = v16 + kHalf;             // [2] stages of K, V codes
+    static constexpr int v16 = k16 + 2 * kHalf;         // two of each
+    static constexpr int raw = v16 + 2 * kHalf;         // [2] stages of K, V codes
     static constexpr int total = raw + 4 * kCodes;
     static constexpr size_t bytes = total + 1024;
     static_assert(bytes + 2048 <= 227 * 1024, "shared memory per CTA");
@@ -71,15 +74,6 @@ IAM_DEV void tmem_ld_wait(uint32_t (&r)[32]) {
                    "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
                    "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
-IAM_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
-        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
-        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
-        : "memory");
-}
 IAM_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(
@@ -110,9 +104,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     using M = Smem<HD>;
     constexpr int PITCH = HD + 4;
     extern __shared__ unsigned char s_raw[];
-    __shared__ __align__(8) uint64_t b_raw_full[2], b_raw_free[2], b_k_ready, b_k_free, b_v_ready, b_v_free, b_q_ready[2], b_s_ready[2],
-        b_p_ready[2], b_o_ready[2];
-    __shared__ float4 s_info[kInfo][kGroups];  // key scale, value scale, 1 if the page is one of the cache's
+    // [2] of the first six by tile, of the others by row tile.  No barrier may complete two phases before its waiter has
+    // looked: S of the next tile can be ready, and its probabilities too, before this one's are waited for, hence one
+    // barrier for each of a row tile's two S.
+    __shared__ __align__(8) uint64_t b_raw_full[2], b_raw_free[2], b_k_ready[2], b_k_free[2], b_v_ready[2], b_v_free[2], b_q_ready[2],
+        b_s_ready[2][2], b_p_ready[2][2], b_o_done[2];
+    __shared__ float4 s_info[kInfo][kGroups];  // key scale, value scale, 1 if the page is one of the cache's, log2 of the value scale
     __shared__ uint32_t s_tmem;
     __shared__ int s_last;
     unsigned char* smem = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
@@ -124,14 +121,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&b_raw_full[i], kGroups);
             mbar_init(&b_raw_free[i], 4);
             mbar_init(&b_q_ready[i], 4);
-            mbar_init(&b_s_ready[i], 1);
-            mbar_init(&b_p_ready[i], 4);
-            mbar_init(&b_o_ready[i], 1);
+            mbar_init(&b_s_ready[i][0], 1);
+            mbar_init(&b_s_ready[i][1], 1);
+            mbar_init(&b_p_ready[i][0], 4);
+            mbar_init(&b_p_ready[i][1], 4);
+            mbar_init(&b_o_done[i], 1);
+            mbar_init(&b_k_ready[i], 4);
+            mbar_init(&b_k_free[i], 1);
+            mbar_init(&b_v_ready[i], 4);
+            mbar_init(&b_v_free[i], 1);
         }
-        mbar_init(&b_k_ready, 4);
-        mbar_init(&b_k_free, 1);
-        mbar_init(&b_v_ready, 4);
-        mbar_init(&b_v_free, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) {
@@ -142,7 +141,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    const uint32_t tm_s[2] = {tmem, tmem + kTile}, tm_o[2] = {tmem + 2 * kTile, tmem + 2 * kTile + HD};
+    // S of row tile i and the j-th tile that it sees, O of row tile i
+    auto tm_s = [&](int i, int j) { return tmem + (uint32_t)((2 * i + (j & 1)) * kTile); };
+    auto tm_o = [&](int i) { return tmem + (uint32_t)(4 * kTile + i * HD); };
 
     const Plan plan{p.s.plan};
     const int items = plan.items();
@@ -186,7 +187,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(b);
     };
 
-    if (warp == 13) {  // ---- copies: lane g has group g of every tile
+    // The registers of a block of 16 warps, 128 a thread, go where they are needed: 152 for the softmax, 104 for the
+    // conversion and the rest (512 for the four warps that share a scheduler, as at the launch).
+    if (warp >= 12) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    else if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    if (warp >= 14) {
+    } else if (warp == 13) {  // ---- copies: lane g has group g of every tile
         for (int n = 0; u < u1; close()) {
             open();
             const int32_t* table = p.c.block_table + (size_t)w.seq * p.c.max_pages;
@@ -205,7 +212,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         id = -1;
                     }
                     const size_t slot = (size_t)id * kvh + w.head;
-                    if (id >= 0) s_info[n % kInfo][lane] = make_float4(__ldg(p.c.k_scale + slot), __ldg(p.c.v_scale + slot), 1.0f, 0.0f);
+                    if (id >= 0) {
+                        const float vs = __ldg(p.c.v_scale + slot);
+                        s_info[n % kInfo][lane] = make_float4(__ldg(p.c.k_scale + slot), vs, 1.0f, __log2f(vs));
+                    }
                     else s_info[n % kInfo][lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     mbar_expect_tx(&b_raw_full[st], id >= 0 ? 2 * kKv8Group * HD : 0);
                     if (id >= 0) {
@@ -221,26 +231,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 12) {  // ---- products
         constexpr uint32_t kDescS = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kQ >> 4) << 24);
         constexpr uint32_t kDescO = (1u << 4) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kQ >> 4) << 24);
-        int n = 0, piece = 0;
-        int n1 = 0, piece1 = 0;  // tiles and pieces that had a second row tile
+        int n = -1, piece = 0;  // n: the tile (of all) whose values are next
+        int s1 = 0, n1 = 0, piece1 = 0;  // of the second row tile: scores, values and pieces so far
         for (; u < u1; close(), ++piece) {
             open();
             const bool two = w.it.n_rows > kQ;
-            auto scores = [&](int i) {  // row tile i times the tile's keys
+            auto scores = [&](int i, int c, int j) {  // row tile i, its c-th, times the keys of tile j (of all)
                 if (lane == 0) {
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k)
-                        tc_mma(tm_s[i], sw128_desc(smem + M::q + i * M::kQBytes + (k >> 2) * (kQ * 128)) + 2u * (k & 3),
-                               sw128_desc(smem + M::k16 + (k >> 2) * (kTile * 128)) + 2u * (k & 3), kDescS, k > 0);
-                    tc_commit(&b_s_ready[i]);
+                        tc_mma(tm_s(i, c), sw128_desc(smem + M::q + i * M::kQBytes + (k >> 2) * (kQ * 128)) + 2u * (k & 3),
+                               sw128_desc(smem + M::k16 + (j & 1) * M::kHalf + (k >> 2) * (kTile * 128)) + 2u * (k & 3), kDescS, k > 0);
+                    tc_commit(&b_s_ready[i][c & 1]);
                 }
             };
-            auto values = [&](int i, bool first) {
+            auto values = [&](int i, int c, int j, bool first) {
                 if (lane == 0) {
 #pragma unroll
                     for (int k = 0; k < kTile / 16; ++k)
-                        tc_mma_ts(tm_o[i], tm_s[i] + 8 * k, sw128_desc(smem + M::v16 + (k >> 2) * (HD * 128)) + 2u * (k & 3), kDescO,
-                                  !first || k > 0);
+                        tc_mma_ts(tm_o(i), tm_s(i, c) + 8 * k, sw128_desc(smem + M::v16 + (j & 1) * M::kHalf) + 2u * k, kDescO, !first || k > 0);
+                    tc_commit(&b_o_done[i]);
                 }
             };
             auto commit = [&](uint64_t* b) {
@@ -248,36 +258,29 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             wait(&b_q_ready[0], piece);
             if (two) wait(&b_q_ready[1], piece1++);
-            wait(&b_k_ready, n);
-            tc_fence_after();
-            scores(0);
-            if (two) scores(1);
-            commit(&b_k_free);
-            for (int j = 0; j < w.n_tiles; ++j, ++n) {
-                const bool more = j + 1 < w.n_tiles;
-                wait(&b_v_ready, n);
-                wait(&b_p_ready[0], n);
-                tc_fence_after();
-                values(0, j == 0);
-                if (more) {
-                    wait(&b_k_ready, n + 1);
+            for (int j = -1; j < w.n_tiles; ++j) {
+                // the next tile's scores go over the probabilities of the tile before this one, whose products were
+                // issued earlier: the tensor cores take them in order
+                if (j + 1 < w.n_tiles) {
+                    wait(&b_k_ready[(n + 1) & 1], (n + 1) >> 1);
                     tc_fence_after();
-                    scores(0);
-                } else {
-                    commit(&b_o_ready[0]);
+                    scores(0, n + 1, n + 1);
+                    if (two) scores(1, s1++, n + 1);
+                    commit(&b_k_free[(n + 1) & 1]);
                 }
-                if (two) {
-                    wait(&b_p_ready[1], n1++);
+                if (j >= 0) {
+                    wait(&b_v_ready[n & 1], n >> 1);
+                    wait(&b_p_ready[0][n & 1], n >> 1);
                     tc_fence_after();
-                    values(1, j == 0);
+                    values(0, n, n, j == 0);
+                    if (two) {
+                        wait(&b_p_ready[1][n1 & 1], n1 >> 1);
+                        tc_fence_after();
+                        values(1, n1++, n, j == 0);
+                    }
+                    commit(&b_v_free[n & 1]);
                 }
-                commit(&b_v_free);
-                if (more) {
-                    if (two) scores(1);
-                    commit(&b_k_free);
-                } else if (two) {
-                    commit(&b_o_ready[1]);
-                }
+                if (j + 1 < w.n_tiles) ++n;
             }
             __syncwarp();
         }
@@ -290,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const unsigned char* raw_k = smem + M::raw + 2 * st * M::kCodes;
                 const unsigned char* raw_v = raw_k + M::kCodes;
                 wait(&b_raw_full[st], n >> 1);
-                wait(&b_k_free, n + 1);
+                wait(&b_k_free[st], (n >> 1) + 1);
                 // keys: 16 codes of a token to 32 bytes of its row; four lanes take half of a token's 128, so that the
                 // stores meet no bank twice
                 constexpr int PIECES = HD / 16;  // of a token
@@ -305,14 +308,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     codes_to_half<FMT>(q.y, a.z, a.w);
                     codes_to_half<FMT>(q.z, b.x, b.y);
                     codes_to_half<FMT>(q.w, b.z, b.w);
-                    unsigned char* to = smem + M::k16 + (c >> 2) * (kTile * 128) + row * 128;
+                    unsigned char* to = smem + M::k16 + st * M::kHalf + (c >> 2) * (kTile * 128) + row * 128;
                     const int piece = (c & 3) * 2;
                     *reinterpret_cast<uint4*>(to + ((piece ^ (row & 7)) << 4)) = a;
                     *reinterpret_cast<uint4*>(to + (((piece + 1) ^ (row & 7)) << 4)) = b;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                give(&b_k_ready);
-                wait(&b_v_free, n + 1);
+                give(&b_k_ready[st]);
+                wait(&b_v_free[st], (n >> 1) + 1);
                 // values: 4 dims of 8 tokens to 4 rows of 16 bytes; lanes take the tokens in turn, so that neither
                 // reads nor stores meet a bank twice
                 constexpr int WORDS = HD / 4;
@@ -337,15 +340,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                         codes_to_half<FMT>(__byte_perm(v[2 * k], v[2 * k + 1], 0x5140), h[0][k], h[1][k]);
                         codes_to_half<FMT>(__byte_perm(v[2 * k], v[2 * k + 1], 0x7362), h[2][k], h[3][k]);
                     }
-                    unsigned char* to = smem + M::v16 + (t8 >> 3) * (HD * 128);
+                    unsigned char* to = smem + M::v16 + st * M::kHalf;
 #pragma unroll
                     for (int d = 0; d < 4; ++d) {
                         const int row = word * 4 + d;
-                        *reinterpret_cast<uint4*>(to + row * 128 + (((t8 & 7) ^ (row & 7)) << 4)) = make_uint4(h[d][0], h[d][1], h[d][2], h[d][3]);
+                        *reinterpret_cast<uint4*>(to + row * 128 + ((t8 ^ (row & 7)) << 4)) = make_uint4(h[d][0], h[d][1], h[d][2], h[d][3]);
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                give(&b_v_ready);
+                give(&b_v_ready[st]);
                 give(&b_raw_free[st]);
             }
         }
@@ -353,8 +356,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int i = warp >> 2;                       // row tile
         const int row = tid & (kQ - 1);                // of the row tile: this thread's lane of tensor memory
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tm_s[i] + lanes, to = tm_o[i] + lanes;
-        int n = 0, ni = 0, piece = 0;  // tiles; tiles and pieces that had this row tile
+        const uint32_t to = tm_o(i) + lanes;
+        int n = 0, ni = 0;  // tiles; tiles that had this row tile
         for (; u < u1; close()) {
             open();
             const int mine = i * kQ + row;
@@ -391,7 +394,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             float m = -INFINITY, l = 0.0f, unit = 0.0f;
             if (!tile_there) n += w.n_tiles;
             for (int j = 0; tile_there && j < w.n_tiles; ++j, ++n, ++ni) {
-                wait(&b_s_ready[i], ni);
+                wait(&b_s_ready[i][ni & 1], ni >> 1);
+                const uint32_t ts = tm_s(i, ni) + lanes;
                 tc_fence_after();
                 const int t0 = w.t_first + j * kTile;
                 const float4* info = s_info[n % kInfo];
@@ -407,98 +411,98 @@ __global__ void __launch_bounds__(kThreads, 1)
                 auto seen = [&](int t, int k) {
                     return info[k].z != 0.0f && t <= pos && t < w.r.cap && (p.window == 0 || t > pos - p.window);
                 };
-                // the row's maximum
-                float mx = -INFINITY;
-                uint32_t s[2][32];
-                tmem_ld32(ts, s[0]);
+                const bool grown = vmax > unit;
+                const float new_unit = grown ? vmax : unit;
+                // The usual tile: every row sees all of it, and the value scales are close enough to go into the
+                // exponent (below); both loops are kept free of the other case's work.
+                const bool plain = whole && vmin >= new_unit * 0x1p-20f && new_unit > 0.0f;
+                const float unit_log = __log2f(new_unit) - kLiftLog;
+                auto tile = [&](auto is_plain) {
+                    constexpr bool PLAIN = decltype(is_plain)::value;
+                    // the row's scores, and their maximum
+                    uint32_t s[2][32];
+                    tmem_ld32(ts, s[0]);
+                    tmem_ld32(ts + 32, s[1]);
+                    tmem_ld_wait(s[0]);
+                    tmem_ld_wait(s[1]);
+                    float mx = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t(&x)[32] = s[c & 1];
-                    tmem_ld_wait(x);
-                    if (c < 3) tmem_ld32(ts + 32 * (c + 1), s[(c + 1) & 1]);
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const float f = fminf(info[2 * c + k].x * rf, 3.402823466e38f);
+                    for (int k = 0; k < kGroups; ++k) {
+                        uint32_t* x = s[k >> 1] + 16 * (k & 1);
+                        const float f = fminf(info[k].x * rf, 3.402823466e38f);
                         float gm = -INFINITY;
-                        if (whole) {
 #pragma unroll
-                            for (int e = 0; e < 16; e += 2)
-                                gm = fmaxf(gm, fmaxf(__uint_as_float(x[16 * k + e]), __uint_as_float(x[16 * k + e + 1])));
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                if (seen(t0 + 32 * c + 16 * k + e, 2 * c + k)) gm = fmaxf(gm, __uint_as_float(x[16 * k + e]));
+                        for (int e = 0; e < 16; e += 2) {
+                            if (!PLAIN) {
+                                if (!seen(t0 + 16 * k + e, k)) x[e] = 0xff800000u;
+                                if (!seen(t0 + 16 * k + e + 1, k)) x[e + 1] = 0xff800000u;
+                            }
+                            gm = fmaxf(gm, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
                         }
                         mx = fmaxf(mx, gm == -INFINITY ? gm : gm * f);
                     }
-                }
-                // The reference follows the maximum with a lag: powers of up to 2^kLag are as exact, and O is
-                // rarely rewritten.  O is in units of the largest value scale so far.
-                const bool grown = vmax > unit;
-                const bool raise = mx > m + kLag || (m == -INFINITY && mx > -INFINITY);
-                if (__any_sync(0xffffffffu, raise) || grown) {
-                    const float ref = raise ? mx : m;
-                    const float fm = raise ? (m == -INFINITY ? 0.0f : ex2(m - ref)) : 1.0f;
-                    const float fo = fm * (grown ? __fdividef(unit, vmax) : 1.0f);
-                    l *= fm;
-                    m = ref;
-                    unit = grown ? vmax : unit;
-                    if (j > 0) {
+                    // The reference follows the maximum with a lag: powers of up to 2^kLag are as exact, and O is
+                    // rarely rewritten.  O is in units of the largest value scale so far.
+                    const bool raise = mx > m + kLag || (m == -INFINITY && mx > -INFINITY);
+                    if (__any_sync(0xffffffffu, raise) || grown) {
+                        const float fm = raise ? (m == -INFINITY ? 0.0f : ex2(m - mx)) : 1.0f;
+                        const float fo = fm * (grown ? __fdividef(unit, vmax) : 1.0f);
+                        l *= fm;
+                        m = raise ? mx : m;
+                        if (j > 0) {
+                            wait(&b_o_done[i], ni - 1);  // the products of the tile before are in
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < HD / 16; ++c) {
+                                uint32_t x[16];
+                                tmem_ld16(to + 16 * c, x);
 #pragma unroll
-                        for (int c = 0; c < HD / 32; ++c) {
-                            uint32_t(&x)[32] = s[c & 1];
-                            tmem_ld32(to + 32 * c, x);
-                            tmem_ld_wait(x);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * fo);
-                            tmem_st32(to + 32 * c, x);
-                        }
-                        tmem_st_wait();
-                    }
-                }
-                const float ref = m == -INFINITY ? 0.0f : m;
-                // powers, rounded to fp16 with the group's value scale (relative to the unit) and the lift in them; the
-                // sum takes both out again, so they are left to a product where they would underflow
-                const bool folded = unit > 0.0f && vmin >= unit * 0x1p-20f;
-                tmem_ld32(ts, s[0]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t(&x)[32] = s[c & 1];
-                    tmem_ld_wait(x);
-                    if (c < 3) tmem_ld32(ts + 32 * (c + 1), s[(c + 1) & 1]);
-                    uint32_t h[16];
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const float4 g = info[2 * c + k];
-                        const float f = fminf(g.x * rf, 3.402823466e38f);
-                        const float ratio = unit > 0.0f ? __fdividef(g.y, unit) * kLift : 0.0f;
-                        const float bias = folded ? __log2f(ratio) - ref : -ref;
-                        float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            float y = fmaf(__uint_as_float(x[16 * k + e]), f, bias);
-                            if (!whole && !seen(t0 + 32 * c + 16 * k + e, 2 * c + k)) y = -INFINITY;
-                            const float v = ex2(y);
-                            sum[e & 1] += v;
-                            x[16 * k + e] = __float_as_uint(v);
-                        }
-                        l = fmaf(sum[0] + sum[1], folded ? __frcp_rn(ratio) : 1.0f, l);
-                        const float after = folded ? 1.0f : ratio;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            float a = __uint_as_float(x[16 * k + 2 * e]), b = __uint_as_float(x[16 * k + 2 * e + 1]);
-                            if (!folded) {
-                                a *= after;
-                                b *= after;
+                                for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * fo);
+                                tmem_st16(to + 16 * c, x);
                             }
-                            h[8 * k + e] = cvt_h2(a, b);
                         }
                     }
-                    tmem_st16(ts + 16 * c, h);  // over scores that have been read
-                }
+                    const float ref = m == -INFINITY ? 0.0f : m;
+                    // powers, rounded to fp16 with the group's value scale (relative to the unit) and the lift in them; a
+                    // plain tile has both in the exponent and takes them out of the sum again
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t h[16];
+#pragma unroll
+                        for (int k = 2 * c; k < 2 * c + 2; ++k) {
+                            const uint32_t* x = s[c] + 16 * (k & 1);
+                            const float4 g = info[k];
+                            const float f = fminf(g.x * rf, 3.402823466e38f);
+                            const float lift = g.w - unit_log, bias = PLAIN ? lift - ref : -ref;
+                            const float ratio = PLAIN || new_unit == 0.0f ? 0.0f : __fdividef(g.y, new_unit) * (float)(1 << kLiftLog);
+                            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+                            for (int e = 0; e < 16; e += 2) {
+                                const float xa = __uint_as_float(x[e]), xb = __uint_as_float(x[e + 1]);
+                                float a = ex2(fmaf(xa, f, bias)), b = ex2(fmaf(xb, f, bias));
+                                if (!PLAIN) {  // (-inf times a scale of 0 is no -inf)
+                                    a = xa == -INFINITY ? 0.0f : a;
+                                    b = xb == -INFINITY ? 0.0f : b;
+                                }
+                                sum[0] += a;
+                                sum[1] += b;
+                                if (!PLAIN) {
+                                    a *= ratio;
+                                    b *= ratio;
+                                }
+                                h[8 * (k & 1) + e / 2] = cvt_h2(a, b);
+                            }
+                            l = fmaf(sum[0] + sum[1], PLAIN ? ex2(-lift) : 1.0f, l);
+                        }
+                        tmem_st16(ts + 16 * c, h);  // over the scores, which are in registers
+                    }
+                };
+                if (plain) tile(std::true_type{});
+                else tile(std::false_type{});
+                unit = new_unit;
                 tmem_st_wait();
                 tc_fence_before();
-                give(&b_p_ready[i]);
+                give(&b_p_ready[i][ni & 1]);
             }
             // ---- results, or this CTA's part of them
             const bool complete = w.tile == 0 && w.n_tiles == w.item1 - w.item0;
@@ -506,9 +510,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             constexpr int PART = kRows * PITCH;
             float* part = p.s.part + (size_t)(2 * blockIdx.x + ((int)blockIdx.x == cta0 ? 1 : 0)) * PART;
             if (tile_there) {
-                wait(&b_o_ready[i], piece++);
+                wait(&b_o_done[i], ni - 1);
                 tc_fence_after();
-                const float scale = unit * (1.0f / kLift);
+                const float scale = unit * (1.0f / (1 << kLiftLog));
 #pragma unroll
                 for (int c = 0; c < HD / 32; ++c) {
                     uint32_t x[32];
