@@ -2,10 +2,10 @@
 // queries, head_dim 64 and 128).
 //
 // A CTA holds two tiles of 128 query rows and walks the tokens 64 at a time.  Scores S = Q K^T and values O += P V are
-// tcgen05.mma (fp16 products, fp32 sums in tensor memory: for each row tile two S, with P over it as the left
-// operand, and O: 512 columns).  S of the next tokens is computed while the softmax works on this one's, so the
-// softmax, which bounds the kernel, never waits for it (one S of 128 tokens, which it waits for, took 1.2 times as
-// long).  The codes become fp16 in shared memory once for both row tiles.  By warp:
+// tcgen05.mma (fp16 products, fp32 sums; in tensor memory, for each row tile, S, two tiles of probabilities as left
+// operands, and O: 512 columns).  No product is written over what another one in flight may read: the tensor cores
+// keep the order of products of one shape only.  S of the next tokens is computed as soon as the softmax has this
+// one's in registers.  The codes become fp16 in shared memory once for both row tiles.  By warp:
 //   0..3, 4..7   softmax of row tile 0, 1: a thread owns a row, so maxima and sums need no exchange
 //   8..11        codes to fp16: keys as they lie, values turned so that a dim's tokens are adjacent (both operands
 //                are then K-major with the 128-byte swizzle)
@@ -105,10 +105,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int PITCH = HD + 4;
     extern __shared__ unsigned char s_raw[];
     // [2] of the first six by tile, of the others by row tile.  No barrier may complete two phases before its waiter has
-    // looked: S of the next tile can be ready, and its probabilities too, before this one's are waited for, hence one
-    // barrier for each of a row tile's two S.
+    // looked: a row tile's next probabilities can be ready before this one's are waited for, hence two barriers.
     __shared__ __align__(8) uint64_t b_raw_full[2], b_raw_free[2], b_k_ready[2], b_k_free[2], b_v_ready[2], b_v_free[2], b_q_ready[2],
-        b_s_ready[2][2], b_p_ready[2][2], b_o_done[2];
+        b_s_ready[2], b_s_free[2], b_p_ready[2][2], b_o_done[2];
     __shared__ float4 s_info[kInfo][kGroups];  // key scale, value scale, 1 if the page is one of the cache's, log2 of the value scale
     __shared__ uint32_t s_tmem;
     __shared__ int s_last;
@@ -121,8 +120,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&b_raw_full[i], kGroups);
             mbar_init(&b_raw_free[i], 4);
             mbar_init(&b_q_ready[i], 4);
-            mbar_init(&b_s_ready[i][0], 1);
-            mbar_init(&b_s_ready[i][1], 1);
+            mbar_init(&b_s_ready[i], 1);
+            mbar_init(&b_s_free[i], 4);
             mbar_init(&b_p_ready[i][0], 4);
             mbar_init(&b_p_ready[i][1], 4);
             mbar_init(&b_o_done[i], 1);
@@ -141,8 +140,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    // S of row tile i and the j-th tile that it sees, O of row tile i
-    auto tm_s = [&](int i, int j) { return tmem + (uint32_t)((2 * i + (j & 1)) * kTile); };
+    // of row tile i: S, the probabilities of the c-th tile that it sees, and O
+    auto tm_s = [&](int i) { return tmem + (uint32_t)(i * kTile); };
+    auto tm_p = [&](int i, int c) { return tmem + (uint32_t)(2 * kTile + (2 * i + (c & 1)) * (kTile / 2)); };
     auto tm_o = [&](int i) { return tmem + (uint32_t)(4 * kTile + i * HD); };
 
     const Plan plan{p.s.plan};
@@ -231,25 +231,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 12) {  // ---- products
         constexpr uint32_t kDescS = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kQ >> 4) << 24);
         constexpr uint32_t kDescO = (1u << 4) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kQ >> 4) << 24);
-        int n = -1, piece = 0;  // n: the tile (of all) whose values are next
-        int s1 = 0, n1 = 0, piece1 = 0;  // of the second row tile: scores, values and pieces so far
+        // (descriptors count in 16 bytes; building each anew took the issuing thread longer than the products)
+        const uint64_t desc_q = sw128_desc(smem + M::q), desc_k = sw128_desc(smem + M::k16), desc_v = sw128_desc(smem + M::v16);
+        int n = 0, piece = 0;  // n: the tile (of all) whose values are next
+        int f0 = 0, f1 = 0, n1 = 0, piece1 = 0;  // tiles that left S; values and pieces of the second row tile
         for (; u < u1; close(), ++piece) {
             open();
             const bool two = w.it.n_rows > kQ;
-            auto scores = [&](int i, int c, int j) {  // row tile i, its c-th, times the keys of tile j (of all)
+            auto scores = [&](int i, int j) {  // row tile i times the keys of tile j (of all)
                 if (lane == 0) {
+                    const uint64_t q = desc_q + (uint64_t)(i * (M::kQBytes >> 4)), keys = desc_k + (uint64_t)((j & 1) * (M::kHalf >> 4));
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k)
-                        tc_mma(tm_s(i, c), sw128_desc(smem + M::q + i * M::kQBytes + (k >> 2) * (kQ * 128)) + 2u * (k & 3),
-                               sw128_desc(smem + M::k16 + (j & 1) * M::kHalf + (k >> 2) * (kTile * 128)) + 2u * (k & 3), kDescS, k > 0);
-                    tc_commit(&b_s_ready[i][c & 1]);
+                        tc_mma(tm_s(i), q + (uint64_t)(((k >> 2) * (kQ * 128) >> 4) + 2 * (k & 3)),
+                               keys + (uint64_t)(((k >> 2) * (kTile * 128) >> 4) + 2 * (k & 3)), kDescS, k > 0);
+                    tc_commit(&b_s_ready[i]);
                 }
             };
-            auto values = [&](int i, int c, int j, bool first) {
+            auto values = [&](int i, int c, int j, bool first) {  // its c-th probabilities times the values of tile j
                 if (lane == 0) {
+                    const uint64_t vals = desc_v + (uint64_t)((j & 1) * (M::kHalf >> 4));
 #pragma unroll
                     for (int k = 0; k < kTile / 16; ++k)
-                        tc_mma_ts(tm_o(i), tm_s(i, c) + 8 * k, sw128_desc(smem + M::v16 + (j & 1) * M::kHalf) + 2u * k, kDescO, !first || k > 0);
+                        tc_mma_ts(tm_o(i), tm_p(i, c) + 8 * k, vals + (uint64_t)(2 * k), kDescO, !first || k > 0);
                     tc_commit(&b_o_done[i]);
                 }
             };
@@ -258,29 +262,37 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             wait(&b_q_ready[0], piece);
             if (two) wait(&b_q_ready[1], piece1++);
-            for (int j = -1; j < w.n_tiles; ++j) {
-                // the next tile's scores go over the probabilities of the tile before this one, whose products were
-                // issued earlier: the tensor cores take them in order
-                if (j + 1 < w.n_tiles) {
+            wait(&b_k_ready[n & 1], n >> 1);
+            tc_fence_after();
+            scores(0, n);
+            if (two) scores(1, n);
+            commit(&b_k_free[n & 1]);
+            for (int j = 0; j < w.n_tiles; ++j, ++n) {
+                if (j + 1 < w.n_tiles) {  // the next tile's scores, as soon as the softmax has this one's in registers
                     wait(&b_k_ready[(n + 1) & 1], (n + 1) >> 1);
+                    wait(&b_s_free[0], f0++);
                     tc_fence_after();
-                    scores(0, n + 1, n + 1);
-                    if (two) scores(1, s1++, n + 1);
-                    commit(&b_k_free[(n + 1) & 1]);
-                }
-                if (j >= 0) {
-                    wait(&b_v_ready[n & 1], n >> 1);
-                    wait(&b_p_ready[0][n & 1], n >> 1);
-                    tc_fence_after();
-                    values(0, n, n, j == 0);
+                    scores(0, n + 1);
                     if (two) {
-                        wait(&b_p_ready[1][n1 & 1], n1 >> 1);
+                        wait(&b_s_free[1], f1++);
                         tc_fence_after();
-                        values(1, n1++, n, j == 0);
+                        scores(1, n + 1);
                     }
-                    commit(&b_v_free[n & 1]);
+                    commit(&b_k_free[(n + 1) & 1]);
+                } else {
+                    wait(&b_s_free[0], f0++);
+                    if (two) wait(&b_s_free[1], f1++);
                 }
-                if (j + 1 < w.n_tiles) ++n;
+                wait(&b_v_ready[n & 1], n >> 1);
+                wait(&b_p_ready[0][n & 1], n >> 1);
+                tc_fence_after();
+                values(0, n, n, j == 0);
+                if (two) {
+                    wait(&b_p_ready[1][n1 & 1], n1 >> 1);
+                    tc_fence_after();
+                    values(1, n1++, n, j == 0);
+                }
+                commit(&b_v_free[n & 1]);
             }
             __syncwarp();
         }
@@ -394,8 +406,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             float m = -INFINITY, l = 0.0f, unit = 0.0f;
             if (!tile_there) n += w.n_tiles;
             for (int j = 0; tile_there && j < w.n_tiles; ++j, ++n, ++ni) {
-                wait(&b_s_ready[i][ni & 1], ni >> 1);
-                const uint32_t ts = tm_s(i, ni) + lanes;
+                wait(&b_s_ready[i], ni);
+                // (S of this tile was issued after the products of the tile before last: their probabilities' place is free)
+                const uint32_t ts = tm_s(i) + lanes, tp = tm_p(i, ni) + lanes;
                 tc_fence_after();
                 const int t0 = w.t_first + j * kTile;
                 const float4* info = s_info[n % kInfo];
@@ -425,6 +438,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_ld32(ts + 32, s[1]);
                     tmem_ld_wait(s[0]);
                     tmem_ld_wait(s[1]);
+                    tc_fence_before();
+                    give(&b_s_free[i]);
                     float mx = -INFINITY;
 #pragma unroll
                     for (int k = 0; k < kGroups; ++k) {
@@ -494,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                             l = fmaf(sum[0] + sum[1], PLAIN ? ex2(-lift) : 1.0f, l);
                         }
-                        tmem_st16(ts + 16 * c, h);  // over the scores, which are in registers
+                        tmem_st16(tp + 16 * c, h);
                     }
                 };
                 if (plain) tile(std::true_type{});
