@@ -82,6 +82,14 @@ IAM_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
         "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
         : "memory");
 }
+// True in one lane of a converged warp, always the same one.  (What the elected lane hands to tcgen05 has to be the same
+// in the whole warp, and known to be: a value that the compiler must first move there costs each instruction some
+// 100 cycles.)
+IAM_DEV bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0u;
+}
 IAM_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 IAM_DEV uint32_t cvt_h2(float lo, float hi) {
     uint32_t r;
@@ -139,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     // of row tile i: S, the probabilities of the c-th tile that it sees, and O
     auto tm_s = [&](int i) { return tmem + (uint32_t)(i * kTile); };
     auto tm_p = [&](int i, int c) { return tmem + (uint32_t)(2 * kTile + (2 * i + (c & 1)) * (kTile / 2)); };
@@ -239,8 +247,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             open();
             const bool two = w.it.n_rows > kQ;
             auto scores = [&](int i, int j) {  // row tile i times the keys of tile j (of all)
-                if (lane == 0) {
-                    const uint64_t q = desc_q + (uint64_t)(i * (M::kQBytes >> 4)), keys = desc_k + (uint64_t)((j & 1) * (M::kHalf >> 4));
+                const int half = __shfl_sync(0xffffffffu, j & 1, 0);
+                const uint64_t q = desc_q + (uint64_t)(i * (M::kQBytes >> 4)), keys = desc_k + (uint64_t)(half * (M::kHalf >> 4));
+                if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k)
                         tc_mma(tm_s(i), q + (uint64_t)(((k >> 2) * (kQ * 128) >> 4) + 2 * (k & 3)),
@@ -249,16 +258,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             };
             auto values = [&](int i, int c, int j, bool first) {  // its c-th probabilities times the values of tile j
-                if (lane == 0) {
-                    const uint64_t vals = desc_v + (uint64_t)((j & 1) * (M::kHalf >> 4));
+                const int half = __shfl_sync(0xffffffffu, j & 1, 0), place = __shfl_sync(0xffffffffu, c & 1, 0);
+                const uint64_t vals = desc_v + (uint64_t)(half * (M::kHalf >> 4));
+                if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < kTile / 16; ++k)
-                        tc_mma_ts(tm_o(i), tm_p(i, c) + 8 * k, vals + (uint64_t)(2 * k), kDescO, !first || k > 0);
+                        tc_mma_ts(tm_o(i), tm_p(i, place) + 8 * k, vals + (uint64_t)(2 * k), kDescO, !first || k > 0);
                     tc_commit(&b_o_done[i]);
                 }
             };
             auto commit = [&](uint64_t* b) {
-                if (lane == 0) tc_commit(b);
+                if (elect_one()) tc_commit(b);
             };
             wait(&b_q_ready[0], piece);
             if (two) wait(&b_q_ready[1], piece1++);
@@ -410,6 +420,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // (S of this tile was issued after the products of the tile before last: their probabilities' place is free)
                 const uint32_t ts = tm_s(i) + lanes, tp = tm_p(i, ni) + lanes;
                 tc_fence_after();
+                uint32_t s[2][32];  // the row's scores
+                tmem_ld32(ts, s[0]);
+                tmem_ld32(ts + 32, s[1]);
                 const int t0 = w.t_first + j * kTile;
                 const float4* info = s_info[n % kInfo];
                 bool all_ok = true;
@@ -430,16 +443,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // exponent (below); both loops are kept free of the other case's work.
                 const bool plain = whole && vmin >= new_unit * 0x1p-20f && new_unit > 0.0f;
                 const float unit_log = __log2f(new_unit) - kLiftLog;
+                tmem_ld_wait(s[0]);
+                tmem_ld_wait(s[1]);
+                tc_fence_before();
+                give(&b_s_free[i]);
                 auto tile = [&](auto is_plain) {
                     constexpr bool PLAIN = decltype(is_plain)::value;
-                    // the row's scores, and their maximum
-                    uint32_t s[2][32];
-                    tmem_ld32(ts, s[0]);
-                    tmem_ld32(ts + 32, s[1]);
-                    tmem_ld_wait(s[0]);
-                    tmem_ld_wait(s[1]);
-                    tc_fence_before();
-                    give(&b_s_free[i]);
                     float mx = -INFINITY;
 #pragma unroll
                     for (int k = 0; k < kGroups; ++k) {
