@@ -40,6 +40,23 @@ IAM_DEV uint32_t encode(float x) {
         return r & 0xffu;
     }
 }
+// Four of them, the first in the lowest byte.
+template <int FMT>
+IAM_DEV uint32_t encode4(float a, float b, float c, float d) {
+    if constexpr (FMT == IAM_KV8_INT8) {
+        return encode<FMT>(a) | encode<FMT>(b) << 8 | encode<FMT>(c) << 16 | encode<FMT>(d) << 24;
+    } else {  // (the conversion itself saturates)
+        a = a == a ? a : 0.0f;
+        b = b == b ? b : 0.0f;
+        c = c == c ? c : 0.0f;
+        d = d == d ? d : 0.0f;
+        uint32_t r;
+        asm("{\n.reg .b16 l, h;\ncvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\ncvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\nmov.b32 %0, {l, h};\n}"
+            : "=r"(r)
+            : "f"(a), "f"(b), "f"(c), "f"(d));
+        return r;
+    }
+}
 template <int FMT>
 IAM_DEV float decode_code(uint32_t b) {
     if constexpr (FMT == IAM_KV8_INT8) return (float)(int8_t)b;
@@ -95,29 +112,11 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(AppendParams
     const int index = first / page + nth;
     const int lo = max(first, (int)page_at), hi = min(r.len, (int)page_at + page);
     if (lo >= hi) return;
-    const int id = p.c.block_table[(size_t)seq * p.c.max_pages + index];
-    if (id < 0 || id >= p.c.n_pages) {
-        if (tid == 0) atomicOr(p.err, kKv8ErrRange);
-        return;
-    }
-    const size_t slot = (size_t)id * p.c.n_kv_heads + head;
-    uint8_t* codes = static_cast<uint8_t*>(which ? p.c.v : p.c.k) + slot * page * hd;
-    float* scale_at = (which ? p.c.v_scale : p.c.k_scale) + slot;
+    // the new values are asked for first; the page they go to is looked up meanwhile
     const iam_rows& rows = p.x[which];
     const T* x = static_cast<const T*>(rows.data) + (size_t)(r.row0 + lo - r.start) * rows.token_stride + head * rows.head_stride;
-    const int held = lo - (int)page_at;  // earlier tokens in the page
-    const float old = held > 0 ? *scale_at : 0.0f;
     const int per_row = hd / VEC, n_vec = (hi - lo) * per_row;
-
     V keep[kAppendKeep];
-    float amax = 0.0f;
-    auto finite_max = [&](const V& v) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float a = fabsf(to_f32(v.v[e]));
-            amax = a <= 3.402823466e38f ? fmaxf(amax, a) : amax;
-        }
-    };
     auto load = [&](int f) {
         const int row = f / per_row, c = f - row * per_row;
         return load_vec<WIDE, T, VEC>(x + (size_t)row * rows.token_stride + c * VEC);
@@ -127,10 +126,39 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(AppendParams
         const int f = tid + k * kAppendThreads;
         if (f < n_vec) keep[k] = load(f);
     }
+    const int id = p.c.block_table[(size_t)seq * p.c.max_pages + index];
+    if (id < 0 || id >= p.c.n_pages) {
+        if (tid == 0) atomicOr(p.err, kKv8ErrRange);
+        return;
+    }
+    const size_t slot = (size_t)id * p.c.n_kv_heads + head;
+    uint8_t* codes = static_cast<uint8_t*>(which ? p.c.v : p.c.k) + slot * page * hd;
+    float* scale_at = (which ? p.c.v_scale : p.c.k_scale) + slot;
+    const int held = lo - (int)page_at;  // earlier tokens in the page
+    const float old = held > 0 ? *scale_at : 0.0f;
+
+    // the largest finite magnitude: of all first (fmaxf passes NaN over), and without the infinities if there are any
+    float amax = 0.0f;
+    auto each = [&](auto&& f) {
 #pragma unroll
-    for (int k = 0; k < kAppendKeep; ++k)
-        if (tid + k * kAppendThreads < n_vec) finite_max(keep[k]);
-    for (int f = tid + kAppendKeep * kAppendThreads; f < n_vec; f += kAppendThreads) finite_max(load(f));
+        for (int k = 0; k < kAppendKeep; ++k)
+            if (tid + k * kAppendThreads < n_vec) f(keep[k]);
+        for (int g = tid + kAppendKeep * kAppendThreads; g < n_vec; g += kAppendThreads) f(load(g));
+    };
+    each([&](const V& v) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) amax = fmaxf(amax, fabsf(to_f32(v.v[e])));
+    });
+    if (amax > 3.402823466e38f) {
+        amax = 0.0f;
+        each([&](const V& v) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float a = fabsf(to_f32(v.v[e]));
+                amax = a <= 3.402823466e38f ? fmaxf(amax, a) : amax;
+            }
+        });
+    }
     amax = warp_max(amax);
     if (lane == 0) s_max[warp] = amax;
     __syncthreads();
@@ -143,11 +171,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(AppendParams
     auto store = [&](int f, const V& v) {
         uint32_t w[VEC / 4];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const uint32_t b = encode<FMT>(to_f32(v.v[e]) * inv);
-            if (e % 4 == 0) w[e / 4] = b;
-            else w[e / 4] |= b << (8 * (e % 4));
-        }
+        for (int e = 0; e < VEC; e += 4)
+            w[e / 4] = encode4<FMT>(to_f32(v.v[e]) * inv, to_f32(v.v[e + 1]) * inv, to_f32(v.v[e + 2]) * inv, to_f32(v.v[e + 3]) * inv);
         uint32_t* to = reinterpret_cast<uint32_t*>(codes + (size_t)held * hd + (size_t)f * VEC);
         if constexpr (VEC == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
         else *to = w[0];
@@ -335,7 +360,14 @@ extern "C" int iam_kv8_attention(iam_kv8_t h, const iam_kv8_cache* cache, int dt
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if ((long long)n_rows * a.gq / 64 + cache->n_seqs > kKv8MaxItems)
         return fail(IAM_ERR_ARG, "kv8: more query rows than one call takes (65536 tiles of 64)");
-    if (rows <= (dtype == IAM_F32 ? 4 : 8)) return kv8_decode_launch(a, dtype, s);
-    if (dtype != IAM_F32 && h->head_dim <= 128 && rows > 64) return kv8_prompt_launch(a, dtype, s);
+    // The decode kernel reads the context once for 8 rows of a KV head (fp32: 4), the rows kernel once for 64, the prompt
+    // kernel once for 256.  Re-reading from L2 costs less than the others' schedule and join up to 4 passes (head_dim 128,
+    // 32 rows: 1 sequence of 8192 tokens 24 us against 59, 32 of 2000 134 against 150), and up to 8 where the sequences'
+    // KV heads do not fill the SMs by themselves (64 rows: 1 x 8192 38 against 76; but 32 x 2000 252 against 168).  The
+    // prompt kernel takes over where there are many rows (512 of 13 x 2 heads: 184 against 261) or heads to fill the SMs
+    // (128 rows of 32 x 8 heads: 218 against 295; of 4 x 8 heads 108 against 105).
+    const long long passes = (rows + (dtype == IAM_F32 ? 3 : 7)) / (dtype == IAM_F32 ? 4 : 8), items = (long long)cache->n_seqs * h->n_kv_heads;
+    if (passes <= 4 || (passes <= 8 && items <= h->sms)) return kv8_decode_launch(a, dtype, s);
+    if (dtype != IAM_F32 && h->head_dim <= 128 && rows > 64 && (rows > 256 || items >= h->sms)) return kv8_prompt_launch(a, dtype, s);
     return kv8_rows_launch(a, dtype, s);
 }

@@ -27,6 +27,7 @@ constexpr int kQ = 128;            // rows of a tile: the MMA's M
 constexpr int kRows = 2 * kQ;
 constexpr int kTile = 64;          // tokens of a unit
 constexpr int kGroups = kTile / kKv8Group;
+constexpr int kMinUnits = 8;       // units of a CTA at least, while there are enough: a context in few parts is joined faster
 constexpr int kThreads = 16 * 32;  // (warps 14 and 15 only complete the last four)
 constexpr int kInfo = 8;           // tiles whose scales are kept: the softmax may be four behind the copies
 constexpr int kLiftLog = 7;        // probabilities (at most 2^kLag) are lifted by 2^kLiftLog before they are rounded to fp16
@@ -157,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int items = plan.items();
     const int per_head = plan.unit()[items];
     const long long total = (long long)per_head * kvh;
-    const long long ctas = min((long long)gridDim.x, total);
+    const long long ctas = min((long long)gridDim.x, (total + kMinUnits - 1) / kMinUnits);
     const bool idle = (long long)blockIdx.x >= ctas;
     const long long u0 = idle ? 0 : total * blockIdx.x / ctas, u1 = idle ? 0 : total * (blockIdx.x + 1) / ctas;
 

@@ -12,6 +12,7 @@ constexpr int kRows = 64;       // query rows of a tile: 16 for each warp
 constexpr int kThreads = 128;
 constexpr int kTile = 64;       // tokens of a work unit
 constexpr int kPerSm = 3;       // CTAs per SM at most (scratch)
+constexpr int kMinUnits = 8;    // units of a CTA at least, while there are enough: a context in few parts is joined faster
 // Row tile (16 rows a warp) times tokens: scores with the queries as A and the tokens as B of m16n8k16, the
 // probabilities (fp16, one or two terms) from the accumulators' own registers as A and the values as B.
 // Codes arrive by cp.async one tile ahead and become fp16 in shared memory once per tile for all warps.
@@ -39,7 +40,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(Kv8Attn p) {
     const int per_head = plan.unit()[items];
     const long long total = (long long)per_head * kvh;
     if (total == 0) return;
-    const long long ctas = min((long long)gridDim.x, total);
+    const long long ctas = min((long long)gridDim.x, (total + kMinUnits - 1) / kMinUnits);
     if (blockIdx.x >= ctas) return;
     const long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
     int item = find_item(plan, items, (int)(u0 % per_head));
@@ -301,28 +302,45 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(Kv8Attn p) {
             if (s_last) {
                 const int parts = cta1 - cta0 + 1;
                 auto part_of = [&](int k) { return p.s.part + (size_t)(2 * (cta0 + k) + (k == 0 ? 1 : 0)) * kRows * PITCH; };
-                for (int row = warp; row < it.n_rows; row += kThreads / 32) {
-                    float top = -INFINITY;
-                    for (int k = lane; k < parts; k += 32) top = fmaxf(top, __ldcg(part_of(k) + row * PITCH + HD));
-                    top = warp_max(top);
-                    const float ref = top == -INFINITY ? 0.0f : top;
-                    float sum = 0.0f, acc[HD / 32];
+                // a thread's 16 bytes of a row from every part, eight parts in flight
+                for (int e = tid; e < it.n_rows * (HD / 4); e += kThreads) {
+                    const int row = e / (HD / 4), d = (e - row * (HD / 4)) * 4;
+                    float top = -INFINITY, sum = 0.0f;
+                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    constexpr int B = 8;
+                    for (int k0 = 0; k0 < parts; k0 += B) {
+                        float2 ml[B];
+                        float4 v[B];
 #pragma unroll
-                    for (int e = 0; e < HD / 32; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-                    for (int k = 0; k < parts; ++k) {
-                        const float* from = part_of(k) + row * PITCH;
-                        const float f = ex2(__ldcg(from + HD) - ref);
-                        sum = fmaf(f, __ldcg(from + HD + 1), sum);
+                        for (int k = 0; k < B; ++k) {
+                            ml[k] = make_float2(-INFINITY, 0.0f);
+                            v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (k0 + k < parts) {
+                                const float* from = part_of(k0 + k) + row * PITCH;
+                                ml[k] = __ldcg(reinterpret_cast<const float2*>(from + HD));
+                                v[k] = __ldcg(reinterpret_cast<const float4*>(from + d));
+                            }
+                        }
+                        const float before = top;
 #pragma unroll
-                        for (int e = 0; e < HD / 32; ++e) acc[e] = fmaf(f, __ldcg(from + e * 32 + lane), acc[e]);
+                        for (int k = 0; k < B; ++k) top = fmaxf(top, ml[k].x);
+                        const float ref = top == -INFINITY ? 0.0f : top, f0 = ex2(before - ref);
+                        sum *= f0;
+                        acc = make_float4(acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0);
+#pragma unroll
+                        for (int k = 0; k < B; ++k) {
+                            const float f = ex2(ml[k].x - ref);
+                            sum = fmaf(f, ml[k].y, sum);
+                            acc = make_float4(fmaf(f, v[k].x, acc.x), fmaf(f, v[k].y, acc.y), fmaf(f, v[k].z, acc.z), fmaf(f, v[k].w, acc.w));
+                        }
                     }
-                    const int rr = rtile * kRows + row;
+                    const int rr = rtile * kRows + row, qh = head * p.gq + rr % p.gq;
                     const size_t to = (size_t)(r.row0 + rr / p.gq);
-                    const int qh = head * p.gq + rr % p.gq;
-#pragma unroll
-                    for (int e = 0; e < HD / 32; ++e) store_result<T>(p, to, qh, e * 32 + lane, acc[e], sum);
-                    if (lane == 0) store_lse(p, to, qh, top, sum);
+                    store_result<T>(p, to, qh, d, acc.x, sum);
+                    store_result<T>(p, to, qh, d + 1, acc.y, sum);
+                    store_result<T>(p, to, qh, d + 2, acc.z, sum);
+                    store_result<T>(p, to, qh, d + 3, acc.w, sum);
+                    if (d == 0) store_lse(p, to, qh, top, sum);
                 }
                 if (tid == 0) p.s.ctr[cta0] = 0;  // ready for the next call
             }

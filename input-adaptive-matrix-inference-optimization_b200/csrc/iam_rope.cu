@@ -74,64 +74,71 @@ struct RopeParams {
     float factor;
 };
 
-// One token per blockIdx.x; its (head, access) items are spread over the block and blockIdx.y.
-// Bound by the bytes: an item is one (pass-through dims) or two (a pair of half-layout vectors)
-// 16-byte loads and as many stores, and the angles cost one reduction in 64 bits and one
-// sincospif per pair and token, shared by all its heads through shared memory.  The angle
+// `group` tokens per blockIdx.x; a thread keeps one place of a head (an access, or a pair of them in the half layout) and
+// walks the (token, head) rows, which are spread over the block and blockIdx.y.  Bound by the bytes; the angles cost one
+// reduction in 64 bits and one sincospif per pair and token, shared by all its heads through shared memory.  The angle
 // in turns is exact to 2^-53 of its size, so a position of 2^31 still has its phase to 2^-24.
 template <class T, bool INTER, bool WIDE>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeParams p) {
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeParams p, int group) {
     constexpr int VEC = WIDE ? 16 / (int)sizeof(T) : INTER ? 2 : 1;  // elements of a rotating access
     constexpr int PASS = WIDE ? VEC : 1;                             // and of one behind them
-    __shared__ __align__(16) float2 cs[kRopeMaxPairs];
-    const int token = blockIdx.x, pairs = p.rot / 2;
-    const int turned = INTER ? p.rot / VEC : pairs / VEC;  // items of a head that rotate
-    const int per_head = turned + (p.head_dim - p.rot) / PASS;
-    const int n_items = (p.heads[0] + p.heads[1]) * per_head;
-    const double pos = (double)p.positions[token];
-    for (int i = threadIdx.x; i < pairs; i += kRopeThreads) {
-        const double t = pos * p.turns[i];
+    __shared__ __align__(16) float2 cs[kRopeMaxPairs];               // [token of the group][pair]
+    const int token0 = blockIdx.x * group, tokens = min(group, p.n_tokens - token0), pairs = p.rot / 2;
+    for (int i = threadIdx.x; i < tokens * pairs; i += kRopeThreads) {
+        const int k = i / pairs;
+        const double t = (double)p.positions[token0 + k] * p.turns[i - k * pairs];
         float s, c;
         sincospif((float)(2.0 * (t - rint(t))), &s, &c);
         cs[i] = make_float2(c * p.factor, s * p.factor);
     }
     __syncthreads();
+    const int turned = INTER ? p.rot / VEC : pairs / VEC;  // places of a head that rotate
+    const int per_head = turned + (p.head_dim - p.rot) / PASS;
+    const int heads = p.heads[0] + p.heads[1], n_rows = tokens * heads;
+    // whole heads to the block's threads; a head with more places than threads in turns
+    const int abreast = max(1, kRopeThreads / per_head);
+    const int my_row = per_head <= kRopeThreads ? threadIdx.x / per_head : 0;
+    if (my_row >= abreast) return;
     using V = Vec<T, VEC>;
-    for (int item = blockIdx.y * kRopeThreads + threadIdx.x; item < n_items; item += gridDim.y * kRopeThreads) {
-        int head = item / per_head;
-        const int j = item - head * per_head;
-        const int which = head >= p.heads[0];
-        head -= which ? p.heads[0] : 0;
-        const iam_rows& ri = p.in[which];
-        const iam_rows& ro = p.out[which];
-        const T* x = static_cast<const T*>(ri.data) + token * ri.token_stride + head * ri.head_stride;
-        T* y = static_cast<T*>(ro.data) + token * ro.token_stride + head * ro.head_stride;
-        if (j >= turned) {  // dims behind the rotated ones
-            const int d = p.rot + (j - turned) * PASS;
-            store_vec<WIDE>(y + d, load_vec<WIDE, T, PASS>(x + d));
-        } else if constexpr (INTER) {
-            const V a = load_vec<WIDE, T, VEC>(x + j * VEC);
-            V o;
+    for (int j = threadIdx.x - my_row * per_head; j < per_head; j += kRopeThreads) {
+#pragma unroll 2
+        for (int row = blockIdx.y * abreast + my_row; row < n_rows; row += gridDim.y * abreast) {
+            const int k = row / heads;
+            int head = row - k * heads;
+            const int which = head >= p.heads[0];
+            head -= which ? p.heads[0] : 0;
+            const iam_rows& ri = p.in[which];
+            const iam_rows& ro = p.out[which];
+            const T* x = static_cast<const T*>(ri.data) + (token0 + k) * ri.token_stride + head * ri.head_stride;
+            T* y = static_cast<T*>(ro.data) + (token0 + k) * ro.token_stride + head * ro.head_stride;
+            const float2* turn = cs + k * pairs;
+            if (j >= turned) {  // dims behind the rotated ones
+                const int d = p.rot + (j - turned) * PASS;
+                store_vec<WIDE>(y + d, load_vec<WIDE, T, PASS>(x + d));
+            } else if constexpr (INTER) {
+                const V a = load_vec<WIDE, T, VEC>(x + j * VEC);
+                V o;
 #pragma unroll
-            for (int e = 0; e < VEC; e += 2) {
-                const float2 t = cs[(j * VEC + e) / 2];
-                const float u = to_f32(a.v[e]), w = to_f32(a.v[e + 1]);
-                o.v[e] = from_f32<T>(u * t.x - w * t.y);
-                o.v[e + 1] = from_f32<T>(w * t.x + u * t.y);
-            }
-            store_vec<WIDE>(y + j * VEC, o);
-        } else {
-            const V a = load_vec<WIDE, T, VEC>(x + j * VEC), b = load_vec<WIDE, T, VEC>(x + pairs + j * VEC);
-            V oa, ob;
+                for (int e = 0; e < VEC; e += 2) {
+                    const float2 t = turn[(j * VEC + e) / 2];
+                    const float u = to_f32(a.v[e]), w = to_f32(a.v[e + 1]);
+                    o.v[e] = from_f32<T>(u * t.x - w * t.y);
+                    o.v[e + 1] = from_f32<T>(w * t.x + u * t.y);
+                }
+                store_vec<WIDE>(y + j * VEC, o);
+            } else {
+                const V a = load_vec<WIDE, T, VEC>(x + j * VEC), b = load_vec<WIDE, T, VEC>(x + pairs + j * VEC);
+                V oa, ob;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float2 t = cs[j * VEC + e];
-                const float u = to_f32(a.v[e]), w = to_f32(b.v[e]);
-                oa.v[e] = from_f32<T>(u * t.x - w * t.y);
-                ob.v[e] = from_f32<T>(w * t.x + u * t.y);
+                for (int e = 0; e < VEC; ++e) {
+                    const float2 t = turn[j * VEC + e];
+                    const float u = to_f32(a.v[e]), w = to_f32(b.v[e]);
+                    oa.v[e] = from_f32<T>(u * t.x - w * t.y);
+                    ob.v[e] = from_f32<T>(w * t.x + u * t.y);
+                }
+                store_vec<WIDE>(y + j * VEC, oa);
+                store_vec<WIDE>(y + pairs + j * VEC, ob);
             }
-            store_vec<WIDE>(y + j * VEC, oa);
-            store_vec<WIDE>(y + pairs + j * VEC, ob);
         }
     }
 }
@@ -140,11 +147,14 @@ template <class T, bool INTER, bool WIDE>
 int launch_rope(const RopeParams& p, int sms, cudaStream_t s) {
     constexpr int VEC = WIDE ? 16 / (int)sizeof(T) : INTER ? 2 : 1;
     const int per_head = (INTER ? p.rot : p.rot / 2) / VEC + (p.head_dim - p.rot) / (WIDE ? VEC : 1);
-    const long long items = (long long)(p.heads[0] + p.heads[1]) * per_head;
-    // few tokens: a token's items over as many blocks as leave one item to a thread
+    const int abreast = std::max(1, kRopeThreads / per_head), heads = p.heads[0] + p.heads[1];
+    // Many tokens: four a block, so that its threads have several rows each; few: a token's heads over as many blocks
+    // as leave a row to a thread
+    const bool many = p.n_tokens >= 8 * sms && 4 * (p.rot / 2) <= kRopeMaxPairs;
+    const int group = many ? 4 : 1;
     long long split = 1;
-    if (p.n_tokens < 2 * sms) split = std::min<long long>((items + kRopeThreads - 1) / kRopeThreads, (2 * sms + p.n_tokens - 1) / p.n_tokens);
-    rope_kernel<T, INTER, WIDE><<<dim3(p.n_tokens, (unsigned)std::max<long long>(1, split)), kRopeThreads, 0, s>>>(p);
+    if (p.n_tokens < 2 * sms) split = std::min<long long>((heads + abreast - 1) / abreast, (2 * sms + p.n_tokens - 1) / p.n_tokens);
+    rope_kernel<T, INTER, WIDE><<<dim3((p.n_tokens + group - 1) / group, (unsigned)std::max<long long>(1, split)), kRopeThreads, 0, s>>>(p, group);
     IAM_CUDA_TRY(cudaGetLastError());
     return IAM_OK;
 }
