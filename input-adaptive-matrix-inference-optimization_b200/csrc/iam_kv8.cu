@@ -9,8 +9,8 @@
 namespace iam {
 namespace {
 
-constexpr int kAppendThreads = 128;
-constexpr int kAppendKeep = 8;  // 16-byte accesses of the new values that a thread keeps between the two passes
+constexpr int kAppendThreads = 256;
+constexpr int kAppendKeep = 4;  // 16-byte accesses of the new values that a thread keeps between the two passes
 
 template <int FMT>
 constexpr float code_top() { return FMT == IAM_KV8_INT8 ? 127.0f : 448.0f; }
@@ -84,25 +84,26 @@ IAM_DEV int slot_base(int cu, int i, int page_log2) { return (cu >> page_log2) +
 // shifts the codes that the page held).  Bound by bytes for prompts (the values are read once and kept
 // in registers up to kAppendKeep accesses a thread), by the chain of dependent loads for single tokens.
 template <class T, int FMT, bool WIDE>
-__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(AppendParams p) {
     constexpr int VEC = WIDE ? 16 / (int)sizeof(T) : 4;
     using V = Vec<T, VEC>;
     __shared__ float s_max[kAppendThreads / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int head = blockIdx.y, which = blockIdx.z;
+    // the KV heads of a page side by side, so that blocks at work together read whole token rows
+    const int lots = 2 * p.c.n_kv_heads, slot_no = blockIdx.x / lots, lot = blockIdx.x - slot_no * lots, head = lot >> 1, which = lot & 1;
     const int page = p.c.page_size, plog = 31 - __clz(page), hd = p.c.head_dim;
-    int seq = blockIdx.x, nth = 0;
+    int seq = slot_no, nth = 0;
     if (p.cu) {  // the sequences whose base is at most this slot
         int count = 0;
         for (int i0 = 0; i0 < p.c.n_seqs; i0 += kAppendThreads) {
             const int i = i0 + tid;
-            const int here = __syncthreads_count(i < p.c.n_seqs && slot_base(p.cu[i], i, plog) <= (int)blockIdx.x);
+            const int here = __syncthreads_count(i < p.c.n_seqs && slot_base(p.cu[i], i, plog) <= slot_no);
             count += here;
             if (here < kAppendThreads) break;
         }
         seq = count - 1;
         if (seq < 0) return;
-        nth = (int)blockIdx.x - slot_base(p.cu[seq], seq, plog);
+        nth = slot_no - slot_base(p.cu[seq], seq, plog);
         if (nth < 0) return;  // (offsets that do not ascend)
     }
     const SeqRows r = seq_rows(p.c, p.cu, p.lens, p.n_rows, seq, p.err);
@@ -113,12 +114,12 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(AppendParams
     const int lo = max(first, (int)page_at), hi = min(r.len, (int)page_at + page);
     if (lo >= hi) return;
     // the new values are asked for first; the page they go to is looked up meanwhile
-    const iam_rows& rows = p.x[which];
+    const iam_rows rows = which ? p.x[1] : p.x[0];
     const T* x = static_cast<const T*>(rows.data) + (size_t)(r.row0 + lo - r.start) * rows.token_stride + head * rows.head_stride;
-    const int per_row = hd / VEC, n_vec = (hi - lo) * per_row;
+    const int row_log = 31 - __clz(hd / VEC), n_vec = (hi - lo) << row_log;  // (head_dim is a power of two)
     V keep[kAppendKeep];
     auto load = [&](int f) {
-        const int row = f / per_row, c = f - row * per_row;
+        const int row = f >> row_log, c = f - (row << row_log);
         return load_vec<WIDE, T, VEC>(x + (size_t)row * rows.token_stride + c * VEC);
     };
 #pragma unroll
@@ -301,10 +302,10 @@ extern "C" int iam_kv8_append(iam_kv8_t h, const iam_kv8_cache* cache, int dtype
     if (!seq_lens_dev) return fail(IAM_ERR_ARG, "kv8: null sequence lengths");
     // slots as numbered on the device (slot_base); one page per sequence when each has one row
     const long long slots = cu_dev ? (long long)n_rows / cache->page_size + 2LL * cache->n_seqs : cache->n_seqs;
-    if (slots > INT32_MAX) return fail(IAM_ERR_ARG, "kv8: too many sequences");
+    if (slots * 2 * cache->n_kv_heads > INT32_MAX) return fail(IAM_ERR_ARG, "kv8: too many sequences");
     AppendParams p{*cache, {*k, *v}, cu_dev, seq_lens_dev, n_rows, (int)slots, h->s.err};
     const bool wide = rows_aligned(*k, elem, 16) && rows_aligned(*v, elem, 16);
-    const dim3 grid((unsigned)slots, cache->n_kv_heads, 2);
+    const dim3 grid((unsigned)(slots * 2 * cache->n_kv_heads));
     DeviceGuard g(h->device);
     IAM_CUDA_TRY(g.err);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
