@@ -228,11 +228,6 @@ class Dense:
 
 # ---------------------------------------------------------------- rotary positions, 8-bit KV cache, log probabilities
 
-class _Rows(ctypes.Structure):
-    """iam_rows (include/iam_b200.h)."""
-    _fields_ = [("data", _vp), ("token_stride", _i64), ("head_stride", _i64)]
-
-
 class _RopeConfig(ctypes.Structure):
     """iam_rope_config."""
     _fields_ = [("head_dim", _i32), ("rot_dim", _i32), ("interleaved", _i32), ("scaling", _i32),
@@ -268,10 +263,14 @@ def _refuse(why):
     raise IamError(IAM_ERR_ARG, why)
 
 
+_DTYPES = {}
+
+
 def _dtype_code(t, what):
-    import torch
-    codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-    code = codes.get(t.dtype)
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    code = _DTYPES.get(t.dtype)
     if code is None:
         _refuse(f"{what}: dtype must be float32, float16 or bfloat16, not {t.dtype}")
     return code
@@ -279,34 +278,47 @@ def _dtype_code(t, what):
 
 def _on(t, device, what, dtype=None, shape=None, contiguous=True):
     """Checks one tensor argument: on CUDA device `device`, of `dtype` and `shape` where given."""
-    if not t.is_cuda or t.device.index != device:
+    if t.get_device() != device:
         _refuse(f"{what}: expected a tensor on cuda:{device}, not {t.device}")
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         _refuse(f"{what}: expected {dtype}, not {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         _refuse(f"{what}: expected shape {tuple(shape)}, not {tuple(t.shape)}")
     if contiguous and not t.is_contiguous():
         _refuse(f"{what}: expected a contiguous tensor")
     return t
 
 
+_Rows = _i64 * 3  # iam_rows (include/iam_b200.h): data, token_stride, head_stride
+
+
 def _rows(t, device, what, dtype, n_rows, n_heads, head_dim):
     """iam_rows of a [rows][heads][head_dim] tensor whose dims of a head are adjacent."""
-    _on(t, device, what, dtype, (n_rows, n_heads, head_dim), contiguous=False)
-    if t.stride(2) != 1:
+    st = t.stride()
+    if t.get_device() != device or t.shape != (n_rows, n_heads, head_dim) or (dtype is not None and t.dtype is not dtype):
+        _on(t, device, what, dtype, (n_rows, n_heads, head_dim), contiguous=False)
+    if st[2] != 1:
         _refuse(f"{what}: the dims of a head must be adjacent")
-    return _Rows(t.data_ptr(), t.stride(0), t.stride(1))
+    return _Rows(t.data_ptr(), st[0], st[1])
+
+
+def _out_rows(t, device, what, dtype, n_rows, n_heads, head_dim):
+    """_rows of an output, whose rows must not share memory (as an expanded tensor's do)."""
+    r = _rows(t, device, what, dtype, n_rows, n_heads, head_dim)
+    if (r[1] == 0 and n_rows > 1) or (r[2] == 0 and n_heads > 1):
+        _refuse(f"{what}: an output's rows must not share memory")
+    return r
 
 
 def _stream_of(device, stream):
+    if stream is not None:
+        return stream.cuda_stream
+    return _torch()._C._cuda_getCurrentRawStream(device)
+
+
+def _torch():
     import torch
-    return (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
-
-
-def _no_overlap(out, what):
-    """An output whose rows share memory (an expanded tensor) would be written by several threads at once."""
-    if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
-        _refuse(f"{what}: an output's rows must not share memory")
+    return torch
 
 
 class Rope:
@@ -350,25 +362,20 @@ class Rope:
     def apply(self, q, positions, out=None, k=None, k_out=None, stream=None):
         """Rotates q [tokens][heads][head_dim] (and k) at int32 `positions` [tokens] into out / k_out
         (None: in place).  Rows may be strided; outputs are their inputs or do not overlap them."""
-        import torch
-        n = q.shape[0]
-        code = _dtype_code(q, "rope q")
-        out = q if out is None else out
-        qi = _rows(q, self.device, "rope q", None, n, q.shape[1], self.head_dim)
-        qo = _rows(out, self.device, "rope out", q.dtype, n, q.shape[1], self.head_dim)
-        _no_overlap(out, "rope out")
+        n, heads, _ = q.shape
+        code, dev, dim, dt = _dtype_code(q, "rope q"), self.device, self.head_dim, q.dtype
+        qi = _rows(q, dev, "rope q", None, n, heads, dim)
+        qo = _out_rows(q if out is None else out, dev, "rope out", dt, n, heads, dim)
         ki = ko = None
         kh = 0
         if k is not None:
             kh = k.shape[1]
-            k_out = k if k_out is None else k_out
-            ki = _rows(k, self.device, "rope k", q.dtype, n, kh, self.head_dim)
-            ko = _rows(k_out, self.device, "rope k_out", q.dtype, n, kh, self.head_dim)
-            _no_overlap(k_out, "rope k_out")
-        _on(positions, self.device, "rope positions", torch.int32, (n,))
-        check(self.lib.iam_rope_apply(self.h, code, n, positions.data_ptr(), q.shape[1], ctypes.byref(qi), ctypes.byref(qo),
-                                      kh, None if ki is None else ctypes.byref(ki), None if ko is None else ctypes.byref(ko),
-                                      _stream_of(self.device, stream)))
+            ki = _rows(k, dev, "rope k", dt, n, kh, dim)
+            ko = _out_rows(k if k_out is None else k_out, dev, "rope k_out", dt, n, kh, dim)
+        _on(positions, dev, "rope positions", _torch().int32, (n,))
+        rc = self.lib.iam_rope_apply(self.h, code, n, positions.data_ptr(), heads, qi, qo, kh, ki, ko, _stream_of(dev, stream))
+        if rc:
+            check(rc)
 
 
 class KV8Cache:
@@ -394,6 +401,7 @@ class KV8Cache:
         self.c = _KV8Cache(formats[k.dtype], k.shape[0], k.shape[2], k.shape[1], k.shape[3], k.data_ptr(), v.data_ptr(),
                            k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), block_table.shape[0],
                            block_table.shape[1])
+        self.ref = ctypes.byref(self.c)
 
     @classmethod
     def empty(cls, n_pages, n_kv_heads, page_size, head_dim, block_table, fmt="e4m3"):
@@ -434,41 +442,41 @@ class KV8:
         check(self.lib.iam_kv8_status(self.h))
 
     def _common(self, cache, seq_lens, cu, what):
-        import torch
         if cache.device != self.device:
             _refuse(f"{what}: the cache is on another device than the handle")
-        _on(seq_lens, self.device, what + " seq_lens", torch.int32, (cache.n_seqs,))
+        int32 = _torch().int32
+        _on(seq_lens, self.device, what + " seq_lens", int32, (cache.n_seqs,))
         if cu is not None:
-            _on(cu, self.device, what + " cu", torch.int32, (cache.n_seqs + 1,))
+            _on(cu, self.device, what + " cu", int32, (cache.n_seqs + 1,))
 
     def append(self, cache, k, v, seq_lens, cu=None, stream=None):
         """Rounds k, v [rows][n_kv_heads][head_dim] into their pages; sequence i owns rows cu[i] .. cu[i + 1]
         (None: row i) and they are the last of its seq_lens[i] tokens."""
         self._common(cache, seq_lens, cu, "kv8 append")
-        n = k.shape[0]
+        n, dev = k.shape[0], self.device
         code = _dtype_code(k, "kv8 append k")
-        kr = _rows(k, self.device, "kv8 append k", None, n, self.n_kv_heads, self.head_dim)
-        vr = _rows(v, self.device, "kv8 append v", k.dtype, n, self.n_kv_heads, self.head_dim)
-        check(self.lib.iam_kv8_append(self.h, ctypes.byref(cache.c), code, n, ctypes.byref(kr), ctypes.byref(vr),
-                                      None if cu is None else cu.data_ptr(), seq_lens.data_ptr(),
-                                      _stream_of(self.device, stream)))
+        kr = _rows(k, dev, "kv8 append k", None, n, self.n_kv_heads, self.head_dim)
+        vr = _rows(v, dev, "kv8 append v", k.dtype, n, self.n_kv_heads, self.head_dim)
+        rc = self.lib.iam_kv8_append(self.h, cache.ref, code, n, kr, vr, None if cu is None else cu.data_ptr(),
+                                     seq_lens.data_ptr(), _stream_of(dev, stream))
+        if rc:
+            check(rc)
 
     def attention(self, cache, q, seq_lens, out, cu=None, max_q=0, scale=0.0, window=0, lse=None, stream=None):
         """Causal attention of q [rows][n_heads][head_dim] over the sequences' tokens into `out` (q's dtype);
         lse (fp32 [rows][n_heads]) receives the log of the sums.  max_q: a bound on one sequence's rows."""
-        import torch
         self._common(cache, seq_lens, cu, "kv8 attention")
-        n = q.shape[0]
+        n, dev = q.shape[0], self.device
         code = _dtype_code(q, "kv8 attention q")
-        qr = _rows(q, self.device, "kv8 attention q", None, n, self.n_heads, self.head_dim)
-        ro = _rows(out, self.device, "kv8 attention out", q.dtype, n, self.n_heads, self.head_dim)
-        _no_overlap(out, "kv8 attention out")
+        qr = _rows(q, dev, "kv8 attention q", None, n, self.n_heads, self.head_dim)
+        ro = _out_rows(out, dev, "kv8 attention out", q.dtype, n, self.n_heads, self.head_dim)
         if lse is not None:
-            _on(lse, self.device, "kv8 attention lse", torch.float32, (n, self.n_heads))
-        check(self.lib.iam_kv8_attention(self.h, ctypes.byref(cache.c), code, n, max_q, ctypes.byref(qr),
-                                         None if cu is None else cu.data_ptr(), seq_lens.data_ptr(), scale, window,
-                                         ctypes.byref(ro), None if lse is None else lse.data_ptr(),
-                                         _stream_of(self.device, stream)))
+            _on(lse, dev, "kv8 attention lse", _torch().float32, (n, self.n_heads))
+        rc = self.lib.iam_kv8_attention(self.h, cache.ref, code, n, max_q, qr, None if cu is None else cu.data_ptr(),
+                                        seq_lens.data_ptr(), scale, window, ro, None if lse is None else lse.data_ptr(),
+                                        _stream_of(dev, stream))
+        if rc:
+            check(rc)
 
 
 def logprobs(logits, targets=None, logprob=None, lse=None, entropy=None, rank=None, top_logprob=None, top_index=None,
@@ -480,7 +488,7 @@ def logprobs(logits, targets=None, logprob=None, lse=None, entropy=None, rank=No
     if logits.dim() != 2 or not logits.is_cuda or logits.stride(1) != 1:
         _refuse("logprobs: logits must be [rows][vocab] on a CUDA device, the tokens of a row adjacent")
     n, vocab = logits.shape
-    dev = logits.device.index
+    dev = logits.get_device()
     code = _dtype_code(logits, "logprobs")
     if targets is not None:
         _on(targets, dev, "logprobs targets", torch.int32, (n,))
@@ -499,10 +507,12 @@ def logprobs(logits, targets=None, logprob=None, lse=None, entropy=None, rank=No
             _opt(rank), k, _opt(top_logprob), _opt(top_index), _stream_of(dev, stream))
     lib = load_library()
     if dev == torch.cuda.current_device():
-        check(lib.iam_logprobs(*args))
+        rc = lib.iam_logprobs(*args)
     else:
         with torch.cuda.device(dev):
-            check(lib.iam_logprobs(*args))
+            rc = lib.iam_logprobs(*args)
+    if rc:
+        check(rc)
 
 
 def _opt(t):

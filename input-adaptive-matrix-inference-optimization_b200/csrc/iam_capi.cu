@@ -145,12 +145,15 @@ const char* iam_version(void) { return "iam-b200 0.1 (sm_100a)"; }
 const char* iam_last_error(void) { return g_last_error.c_str(); }
 
 int iam_device_info(int device, int* sm_count, int* cc_major, int* cc_minor) {
-    cudaDeviceProp prop;
-    IAM_CUDA_TRY(cudaGetDeviceProperties(&prop, device));
-    if (sm_count) *sm_count = prop.multiProcessorCount;
-    if (cc_major) *cc_major = prop.major;
-    if (cc_minor) *cc_minor = prop.minor;
-    if (prop.major != 10) return fail(IAM_ERR_UNSUPPORTED, "libiamb200 is built for sm_100a only");
+    // (single attributes: the whole property record takes milliseconds)
+    int sms = 0, major = 0, minor = 0;
+    IAM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    IAM_CUDA_TRY(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+    IAM_CUDA_TRY(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device));
+    if (sm_count) *sm_count = sms;
+    if (cc_major) *cc_major = major;
+    if (cc_minor) *cc_minor = minor;
+    if (major != 10) return fail(IAM_ERR_UNSUPPORTED, "libiamb200 is built for sm_100a only");
     return IAM_OK;
 }
 
