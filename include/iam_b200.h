@@ -411,6 +411,21 @@ int iam_feedforward_forward(iam_model_t m, int layer, const float* h_dev, float 
  * Single-GPU models only (IAM_ERR_UNSUPPORTED for a tensor-parallel rank). */
 int iam_model_prefill(iam_model_t m, const int* tokens_host, int n_tokens, int start_pos, float* logits_dev,
                       int* next_token, void* stream);
+/* Rotary positions of the model from here on: its table of angles is rebuilt from `cfg` (half
+ * layout over the whole head: rot_dim = head_dim = the model's, interleaved 0; else
+ * IAM_ERR_UNSUPPORTED), with the angles in 64 bits.  NULL puts the table of attention.hpp:210-226
+ * back.  Keys already in the cache keep their rotation, so call it before the first token or reset
+ * the caches; every rank of a tensor-parallel group makes the same call.  Synchronises the device;
+ * captured steps stay valid. */
+int iam_model_set_rope(iam_model_t m, const iam_rope_config* cfg);
+/* Scores a text: iam_model_prefill of the n_tokens tokens (with its effects on caches, position and
+ * next token), and for each of them the log probability of a given next token.  targets_dev[t]
+ * (int32, device) is the token whose probability is wanted after tokens_host[0 .. t], negative for
+ * none; the outputs are those of iam_logprobs, one row per token, and follow its rules (any may be
+ * NULL but those of a positive top_k).  Single-GPU models only. */
+int iam_model_score(iam_model_t m, const int* tokens_host, int n_tokens, int start_pos, const int32_t* targets_dev,
+                    float* logprob_dev, float* entropy_dev, int32_t* rank_dev, int top_k, float* top_logprob_dev,
+                    int32_t* top_index_dev, int* next_token, void* stream);
 /* Greedy generation on the device (the decode loop of test_generation.cpp:239-291 without
  * host round trips): step 0 decodes first_token at start_pos, every later step decodes the
  * previous step's argmax; the n_tokens generated ids land in tokens_dev.  Steps after the

@@ -552,6 +552,8 @@ _SIGNATURES.update({
     "iam_attention_forward": [_vp, _i32, _vp, _i32, _f32, _vp, _vp],
     "iam_feedforward_forward": [_vp, _i32, _vp, _f32, _vp, _vp],
     "iam_model_prefill": [_vp, _vp, _i32, _i32, _vp, _vp, _vp],
+    "iam_model_set_rope": [_vp, _vp],
+    "iam_model_score": [_vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp],
     "iam_model_generate": [_vp, _i32, _i32, _i32, _f32, _vp, _vp],
     "iam_model_set_kv": [_vp, _i32, _vp, _vp, _i32, _vp],
     "iam_model_fill_kv_random": [_vp, _i32, ctypes.c_ulonglong, _vp],
@@ -684,6 +686,31 @@ class Model:
         nxt = ctypes.c_int(-1)
         check(self.lib.iam_model_prefill(self.h, arr, len(tokens), start_pos, _ptr(logits), ctypes.byref(nxt),
                                          _stream(stream)))
+        return nxt.value
+
+    def set_rope(self, cfg):
+        """iam_model_set_rope: rotary positions of the model from a Rope.config() (None: its own again)."""
+        check(self.lib.iam_model_set_rope(self.h, None if cfg is None else ctypes.byref(cfg)))
+
+    def score(self, tokens, targets=None, start_pos=0, logprob=None, entropy=None, rank=None, top_logprob=None,
+              top_index=None, stream=None):
+        """iam_model_score: the prompt as in prefill(), and of each of its tokens the log probability, rank,
+        entropy and best alternatives of the next one; targets int32 [tokens] on the device (negative: none),
+        outputs as logprobs().  Returns the greedy next token."""
+        n = len(tokens)
+        k = 0 if top_logprob is None else top_logprob.shape[-1]
+        if (top_logprob is None) != (top_index is None):
+            _refuse("score: top_logprob and top_index come together")
+        torch = _torch()
+        for t, what, dt, shape in ((targets, "targets", torch.int32, (n,)), (logprob, "logprob", torch.float32, (n,)),
+                                   (entropy, "entropy", torch.float32, (n,)), (rank, "rank", torch.int32, (n,)),
+                                   (top_logprob, "top_logprob", torch.float32, (n, k)), (top_index, "top_index", torch.int32, (n, k))):
+            if t is not None:
+                _on(t, t.get_device() if t.is_cuda else 0, "score " + what, dt, shape)
+        arr = (ctypes.c_int * n)(*[int(t) for t in tokens])
+        nxt = ctypes.c_int(-1)
+        check(self.lib.iam_model_score(self.h, arr, n, start_pos, _opt(targets), _opt(logprob), _opt(entropy), _opt(rank), k,
+                                       _opt(top_logprob), _opt(top_index), ctypes.byref(nxt), _stream(stream)))
         return nxt.value
 
     def generate(self, first_token, start_pos, n_tokens, effort, tokens, stream=None):

@@ -16,6 +16,7 @@
 #include <cstring>
 #include <thread>
 #include <fstream>
+#include <functional>
 #include <sstream>
 #include <string>
 #include <vector>
@@ -28,6 +29,7 @@
 #include "iam_dense.h"
 #include "iam_layers.h"
 #include "iam_prefill.h"
+#include "iam_rope.h"
 #include "iam_tp.h"
 
 namespace iam {
@@ -258,6 +260,7 @@ struct iam_model_s {
     uint16_t *pf_hi2 = nullptr, *pf_lo2 = nullptr;  // SiLU(gate) * up as the down product's input
     bool pf_silu_fused = false;  // gate|up rows interleaved in 128-row blocks, SiLU in its epilogue
     unsigned* pf_err = nullptr;
+    float* pf_logits = nullptr;  // [pf_cap][vocab], built by the first iam_model_score
 };
 
 namespace {
@@ -1432,8 +1435,10 @@ int iam_model_forward(iam_model_t m, int token, int pos, float effort, float* lo
     return rc;
 }
 
-int iam_model_prefill(iam_model_t m, const int* tokens_host, int n_tokens, int start_pos, float* logits_dev,
-                      int* next_token, void* stream) {
+// The prompt through every layer, `after` on each chunk's residual stream (its first token and their number), and
+// the last token's logits and argmax: what iam_model_prefill and iam_model_score share.
+static int run_prefill(iam_model_t m, const int* tokens_host, int n_tokens, int start_pos, float* logits_dev, int* next_token, void* stream,
+                       const std::function<int(int, int)>& after) {
     if (!m || !tokens_host) return fail(IAM_ERR_ARG, "iam_model_prefill: null argument");
     if (m->tp_world > 1) return fail(IAM_ERR_UNSUPPORTED, "iam_model_prefill: single-GPU models only");
     const iam_model_config& c = m->cfg;
@@ -1449,6 +1454,7 @@ int iam_model_prefill(iam_model_t m, const int* tokens_host, int n_tokens, int s
     for (int c0 = 0; c0 < n_tokens; c0 += m->pf_cap) {
         last_rows = std::min(m->pf_cap, n_tokens - c0);
         if ((rc = prefill_chunk(m, tokens_host + c0, last_rows, start_pos + c0, s))) return rc;
+        if (after && (rc = after(c0, last_rows))) return rc;
     }
     IAM_CUDA_TRY(cudaMemsetAsync(m->key, 0, sizeof(unsigned long long), s));
     LMHeadParams hp{};
@@ -1475,6 +1481,62 @@ int iam_model_prefill(iam_model_t m, const int* tokens_host, int n_tokens, int s
         IAM_CUDA_TRY(cudaMemcpy(&key, m->key, sizeof(key), cudaMemcpyDeviceToHost));
         *next_token = (int)(0xffffffffu - (unsigned)(key & 0xffffffffull));
     }
+    return IAM_OK;
+}
+
+int iam_model_prefill(iam_model_t m, const int* tokens_host, int n_tokens, int start_pos, float* logits_dev,
+                      int* next_token, void* stream) {
+    return run_prefill(m, tokens_host, n_tokens, start_pos, logits_dev, next_token, stream, nullptr);
+}
+
+int iam_model_score(iam_model_t m, const int* tokens_host, int n_tokens, int start_pos, const int32_t* targets_dev,
+                    float* logprob_dev, float* entropy_dev, int32_t* rank_dev, int top_k, float* top_logprob_dev,
+                    int32_t* top_index_dev, int* next_token, void* stream) {
+    if (!m) return fail(IAM_ERR_ARG, "iam_model_score: null argument");
+    // iam_logprobs' checks before anything is launched
+    int rc = iam_logprobs(nullptr, IAM_F32, 0, m->cfg.vocab, m->cfg.vocab, nullptr, nullptr, nullptr, nullptr, nullptr, top_k, nullptr, nullptr, stream);
+    if (rc) return rc;
+    if (top_k > 0 && (!top_logprob_dev || !top_index_dev)) return fail(IAM_ERR_ARG, "iam_model_score: null top outputs");
+    if (!targets_dev && (logprob_dev || rank_dev)) return fail(IAM_ERR_ARG, "iam_model_score: logprob and rank need targets");
+    const cudaStream_t s = (cudaStream_t)stream;
+    auto rows = [&](int first, int n) -> int {
+        const iam_model_config& c = m->cfg;
+        int r;
+        if (!m->pf_logits && (r = dalloc(m, &m->pf_logits, (size_t)m->pf_cap * c.vocab))) return r;
+        if ((r = prefill_rms_split(m->pf_h, n, c.dim, m->final_norm, c.norm_eps, m->pf_hi, m->pf_lo, s)) ||
+            (r = prefill_gemm(m, m->lm_head, c.vocab, c.dim, n, m->pf_logits, nullptr, s)))
+            return r;
+        auto at = [&](auto* p, size_t per) { return p ? p + per * first : nullptr; };
+        return iam_logprobs(m->pf_logits, IAM_F32, n, c.vocab, c.vocab, at(targets_dev, 1), at(logprob_dev, 1), nullptr, at(entropy_dev, 1),
+                            at(rank_dev, 1), top_k, at(top_logprob_dev, top_k), at(top_index_dev, top_k), stream);
+    };
+    return run_prefill(m, tokens_host, n_tokens, start_pos, nullptr, next_token, stream, rows);
+}
+
+int iam_model_set_rope(iam_model_t m, const iam_rope_config* cfg) {
+    if (!m) return fail(IAM_ERR_ARG, "iam_model_set_rope: null model");
+    std::vector<float> t;
+    if (!cfg) {
+        t = rope_table(m->cfg);
+    } else {
+        const int rc = rope_check(cfg);
+        if (rc) return rc;
+        if (cfg->head_dim != m->cfg.head_dim || cfg->rot_dim != cfg->head_dim || cfg->interleaved)
+            return fail(IAM_ERR_UNSUPPORTED, "iam_model_set_rope: the model rotates its whole head, in the half layout");
+        const int half = cfg->head_dim / 2;
+        std::vector<double> w(half);
+        double factor = 1.0;
+        rope_frequencies(*cfg, w.data(), &factor);
+        t.resize((size_t)m->cfg.max_ctx * cfg->head_dim);
+        for (int p = 0; p < m->cfg.max_ctx; ++p)
+            for (int i = 0; i < half; ++i) {
+                t[((size_t)p * half + i) * 2] = (float)(std::cos(p * w[i]) * factor);
+                t[((size_t)p * half + i) * 2 + 1] = (float)(std::sin(p * w[i]) * factor);
+            }
+    }
+    IAM_CUDA_TRY(cudaSetDevice(m->device));
+    IAM_CUDA_TRY(cudaDeviceSynchronize());
+    IAM_CUDA_TRY(cudaMemcpy(m->rope, t.data(), t.size() * sizeof(float), cudaMemcpyHostToDevice));
     return IAM_OK;
 }
 

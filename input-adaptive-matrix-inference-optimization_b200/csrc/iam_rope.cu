@@ -8,6 +8,7 @@
 #include <cmath>
 #include <new>
 
+#include "iam_rope.h"
 #include "iam_types.cuh"
 
 namespace iam {
@@ -38,7 +39,6 @@ int rope_check(const iam_rope_config* c) {
     return IAM_OK;
 }
 
-// Radians per position of every pair, and the factor on the rotated values.
 void rope_frequencies(const iam_rope_config& c, double* w, double* factor) {
     const int d = c.rot_dim;
     const double lo = c.low_turns > 0 ? c.low_turns : 1.0;
