@@ -233,7 +233,8 @@ int iam_rope_apply(iam_rope_t h, int dtype, int n_tokens, const int32_t* positio
 /* A paged cache of keys and values in 8 bits with one fp32 scale per page and KV head, owned by
  * the caller: codes [n_pages][n_kv_heads][page_size][head_dim], scales [n_pages][n_kv_heads], a
  * value being code * scale.  Sequence i keeps token t in page block_table[i * max_pages + t /
- * page_size], row t % page_size.  The scale of a page is the smallest power of two (at least
+ * page_size], row t % page_size.  At most 2^31 rows of codes (n_pages * n_kv_heads * page_size), and
+ * 2^26 tokens a sequence.  The scale of a page is the smallest power of two (at least
  * 2^-126) that brings every value of the page and head within the largest code (127; 448 for
  * e4m3): dividing by it is exact, so each value is rounded once (to nearest, ties to even), and a
  * page whose scale grows when larger values are appended shifts its older codes. */
@@ -248,7 +249,7 @@ typedef struct {
     int n_seqs, max_pages;
 } iam_kv8_cache;
 typedef struct iam_kv8_s* iam_kv8_t;
-/* A handle owns the scratch of the attention's split context (about 20 to 80 MB, set by head_dim;
+/* A handle owns the scratch of the attention's split context (20 to 60 MB, set by head_dim;
  * never reallocated, so captured graphs keep it) and an error word.  One handle per stream: calls
  * of one handle must not overlap on the GPU, graphs captured with it included. */
 int iam_kv8_create(iam_kv8_t* out, int n_heads, int n_kv_heads, int head_dim, int device);
@@ -268,13 +269,15 @@ int iam_kv8_append(iam_kv8_t h, const iam_kv8_cache* cache, int dtype, int n_row
  * (p - window, p] (window 0: all up to p); query head j reads KV head j / (n_heads / n_kv_heads).
  * scale 0: 1/sqrt(head_dim).  out has q's dtype; lse_dev (may be NULL) [n_rows][n_heads] fp32
  * receives the natural logarithm of the sum of exponentials.  A row that sees nothing (a position
- * below 0) gives 0 and -inf.  max_q: a bound on one sequence's rows, if known (0: n_rows); it
+ * below 0) gives 0 and -inf.  out may be q itself (with its strides).  At most 65536 tiles of 64 rows (n_rows * n_heads /
+ * n_kv_heads / 64 + n_seqs).  max_q: a bound on one sequence's rows, if known (0: n_rows); it
  * chooses the kernel and never the result's meaning.  What stands in a page behind the sequence's
  * last token has no influence. */
 int iam_kv8_attention(iam_kv8_t h, const iam_kv8_cache* cache, int dtype, int n_rows, int max_q, const iam_rows* q,
                       const int32_t* cu_dev, const int32_t* seq_lens_dev, float scale, int window, const iam_rows* out,
                       float* lse_dev, void* stream);
-/* Synchronises the device; IAM_ERR_ARG when a call of `h` since the last iam_kv8_status met a page
+/* Synchronises the device; IAM_ERR_TIMEOUT when a wait of the attention gave up (its results are then
+ * invalid), IAM_ERR_ARG when a call of `h` since the last iam_kv8_status met a page
  * number outside the cache, a sequence longer than its table, a negative length or row offsets
  * that do not ascend within n_rows (such tokens or sequences are skipped); the word is then cleared.
  * Tokens before position 0 (more rows than the sequence has tokens, as in the padding of a batch) are

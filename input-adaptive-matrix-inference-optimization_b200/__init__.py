@@ -612,8 +612,8 @@ class Model:
     """Mirror of MistralModel (model.hpp:84-237) on one device, or one rank of a
     tensor-parallel group (tp=(rank, world, tp_unique_id() of rank 0))."""
 
-    def __init__(self, cfg, h, tp=None):
-        self.cfg, self.h, self.lib = cfg, h, load_library()
+    def __init__(self, cfg, h, tp=None, device=0):
+        self.cfg, self.h, self.lib, self.device = cfg, h, load_library(), device
         self.rank, self.world = (tp[0], tp[1]) if tp else (0, 1)
 
     @classmethod
@@ -625,7 +625,7 @@ class Model:
             check(lib.iam_model_create_random_tp(ctypes.byref(h), ctypes.byref(cfg), seed, device, rank, world, uid))
         else:
             check(lib.iam_model_create_random(ctypes.byref(h), ctypes.byref(cfg), seed, device))
-        return cls(cfg, h, tp)
+        return cls(cfg, h, tp, device)
 
     @classmethod
     def load(cls, weights_dir, cfg, device=0, tp=None):
@@ -637,7 +637,7 @@ class Model:
                                         world, uid))
         else:
             check(lib.iam_model_load(ctypes.byref(h), os.fsencode(weights_dir), ctypes.byref(cfg), device))
-        return cls(cfg, h, tp)
+        return cls(cfg, h, tp, device)
 
     def close(self):
         if self.h:
@@ -706,7 +706,7 @@ class Model:
                                    (entropy, "entropy", torch.float32, (n,)), (rank, "rank", torch.int32, (n,)),
                                    (top_logprob, "top_logprob", torch.float32, (n, k)), (top_index, "top_index", torch.int32, (n, k))):
             if t is not None:
-                _on(t, t.get_device() if t.is_cuda else 0, "score " + what, dt, shape)
+                _on(t, self.device, "score " + what, dt, shape)
         arr = (ctypes.c_int * n)(*[int(t) for t in tokens])
         nxt = ctypes.c_int(-1)
         check(self.lib.iam_model_score(self.h, arr, n, start_pos, _opt(targets), _opt(logprob), _opt(entropy), _opt(rank), k,

@@ -70,7 +70,7 @@ struct AppendParams {
     iam_rows x[2];
     const int32_t* cu;
     const int32_t* lens;
-    int n_rows, n_slots;
+    int n_rows;
     unsigned* err;
 };
 
@@ -207,6 +207,7 @@ int check_cache(const iam_kv8_cache* c) {
         return fail(IAM_ERR_UNSUPPORTED, "kv8: head_dim must be 64, 128 or 256");
     if (c->n_kv_heads <= 0 || c->n_pages <= 0 || c->max_pages <= 0 || c->n_seqs < 0) return fail(IAM_ERR_ARG, "kv8: bad cache sizes");
     if (c->n_kv_heads > 65535) return fail(IAM_ERR_ARG, "kv8: more than 65535 KV heads");
+    if ((long long)c->max_pages * c->page_size > kKv8MaxTokens) return fail(IAM_ERR_UNSUPPORTED, "kv8: a table of more than 2^26 tokens");
     if ((long long)c->n_pages * c->n_kv_heads * c->page_size > INT32_MAX) return fail(IAM_ERR_UNSUPPORTED, "kv8: more than 2^31 rows of codes");
     if (!c->k || !c->v || !c->k_scale || !c->v_scale || (c->n_seqs > 0 && !c->block_table)) return fail(IAM_ERR_ARG, "kv8: null cache array");
     if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16)
@@ -303,7 +304,7 @@ extern "C" int iam_kv8_append(iam_kv8_t h, const iam_kv8_cache* cache, int dtype
     // slots as numbered on the device (slot_base); one page per sequence when each has one row
     const long long slots = cu_dev ? (long long)n_rows / cache->page_size + 2LL * cache->n_seqs : cache->n_seqs;
     if (slots * 2 * cache->n_kv_heads > INT32_MAX) return fail(IAM_ERR_ARG, "kv8: too many sequences");
-    AppendParams p{*cache, {*k, *v}, cu_dev, seq_lens_dev, n_rows, (int)slots, h->s.err};
+    AppendParams p{*cache, {*k, *v}, cu_dev, seq_lens_dev, n_rows, h->s.err};
     const bool wide = rows_aligned(*k, elem, 16) && rows_aligned(*v, elem, 16);
     const dim3 grid((unsigned)(slots * 2 * cache->n_kv_heads));
     DeviceGuard g(h->device);
@@ -348,7 +349,7 @@ extern "C" int iam_kv8_attention(iam_kv8_t h, const iam_kv8_cache* cache, int dt
     a.n_rows = n_rows;
     a.n_heads = h->n_heads;
     a.gq = h->n_heads / h->n_kv_heads;
-    a.window = window;
+    a.window = std::min(window, 1 << 30);  // (beyond every table; position - window stays an int)
     a.scale_log2 = (float)((scale > 0.0f ? (double)scale : 1.0 / std::sqrt((double)h->head_dim)) * 1.4426950408889634074);
     a.q = *q;
     a.out = *out;

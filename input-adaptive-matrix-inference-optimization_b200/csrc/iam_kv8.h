@@ -10,8 +10,9 @@
 namespace iam {
 
 constexpr int kKv8MaxItems = 1 << 16;  // row tiles of one attention call at most
+constexpr int kKv8MaxTokens = 1 << 26; // tokens that a sequence's table can name
 constexpr int kKv8Group = 16;          // tokens that share a page for sure (the smallest page)
-constexpr unsigned kKv8ErrRange = 1u;  // error word: a page, length or row offset out of range
+constexpr unsigned kKv8ErrRange = 1u;  // error word: a page, length or row offset out of range, or more work than a call takes
 constexpr unsigned kKv8ErrWait = 2u;   // a bounded wait gave up
 
 // Scratch of a handle: partial results of row tiles whose context is split over several CTAs, the

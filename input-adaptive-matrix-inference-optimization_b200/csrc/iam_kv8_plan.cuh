@@ -3,6 +3,8 @@
 // that is cut into equal runs, one per CTA.
 #pragma once
 
+#include <climits>
+
 #include "iam_kv8.cuh"
 
 namespace iam {
@@ -80,7 +82,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Kv8Attn p) {
         items = min(items + total, kKv8MaxItems);  // (more only when the row offsets do not ascend)
     }
     __syncthreads();
-    int units = 0;
+    long long units = 0;
     for (int i0 = 0; i0 < items; i0 += kPlanThreads) {
         const int i = i0 + tid;
         int n = 0;
@@ -88,13 +90,15 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Kv8Attn p) {
             const int seq = plan.seq()[i];
             n = item_of<ROWS, TILE>(p, seq_rows(p.c, p.cu, p.lens, p.n_rows, seq, nullptr), plan.rtile()[i]).nt;
         }
-        const int at = units + block_scan(n, s_warp, total);
-        if (i < items) plan.unit()[i] = at;
+        const long long at = units + block_scan(n, s_warp, total);  // (1024 tiles of at most 2^20 units)
+        if (i < items) plan.unit()[i] = (int)min(at, (long long)INT_MAX);
         units += total;
     }
     if (tid == 0) {
-        plan.unit()[items] = units;
-        plan.items() = items;
+        const bool fits = units < INT_MAX;
+        if (!fits) atomicOr(p.s.err, kKv8ErrRange);
+        plan.unit()[fits ? items : 0] = fits ? (int)units : 0;
+        plan.items() = fits ? items : 0;
     }
 }
 

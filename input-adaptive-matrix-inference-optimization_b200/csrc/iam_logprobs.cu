@@ -485,6 +485,7 @@ extern "C" int iam_logprobs(const void* logits_dev, int dtype, int n_rows, int v
                             float* logprob_dev, float* lse_dev, float* entropy_dev, int32_t* rank_dev, int top_k, float* top_logprob_dev,
                             int32_t* top_index_dev, void* stream) {
     if (!dtype_ok(dtype)) return fail(IAM_ERR_ARG, "logprobs: dtype must be IAM_F32, IAM_F16 or IAM_BF16");
+    if (n_rows > 1 << 30) return fail(IAM_ERR_ARG, "logprobs: more than 2^30 rows");
     if (n_rows < 0 || vocab <= 0) return fail(IAM_ERR_ARG, "logprobs: bad sizes");
     if (n_rows > 1 && row_stride < vocab) return fail(IAM_ERR_ARG, "logprobs: rows overlap");
     if (top_k < 0 || top_k > kMaxTop || top_k > vocab) return fail(IAM_ERR_ARG, "logprobs: top_k must be in [0, min(64, vocab)]");

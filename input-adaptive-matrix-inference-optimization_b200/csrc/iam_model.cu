@@ -16,7 +16,7 @@
 #include <cstring>
 #include <thread>
 #include <fstream>
-#include <functional>
+#include <new>
 #include <sstream>
 #include <string>
 #include <vector>
@@ -1437,8 +1437,10 @@ int iam_model_forward(iam_model_t m, int token, int pos, float effort, float* lo
 
 // The prompt through every layer, `after` on each chunk's residual stream (its first token and their number), and
 // the last token's logits and argmax: what iam_model_prefill and iam_model_score share.
+extern "C++" {
+template <class F>
 static int run_prefill(iam_model_t m, const int* tokens_host, int n_tokens, int start_pos, float* logits_dev, int* next_token, void* stream,
-                       const std::function<int(int, int)>& after) {
+                       const F& after) {
     if (!m || !tokens_host) return fail(IAM_ERR_ARG, "iam_model_prefill: null argument");
     if (m->tp_world > 1) return fail(IAM_ERR_UNSUPPORTED, "iam_model_prefill: single-GPU models only");
     const iam_model_config& c = m->cfg;
@@ -1454,7 +1456,7 @@ static int run_prefill(iam_model_t m, const int* tokens_host, int n_tokens, int 
     for (int c0 = 0; c0 < n_tokens; c0 += m->pf_cap) {
         last_rows = std::min(m->pf_cap, n_tokens - c0);
         if ((rc = prefill_chunk(m, tokens_host + c0, last_rows, start_pos + c0, s))) return rc;
-        if (after && (rc = after(c0, last_rows))) return rc;
+        if ((rc = after(c0, last_rows))) return rc;
     }
     IAM_CUDA_TRY(cudaMemsetAsync(m->key, 0, sizeof(unsigned long long), s));
     LMHeadParams hp{};
@@ -1483,10 +1485,11 @@ static int run_prefill(iam_model_t m, const int* tokens_host, int n_tokens, int 
     }
     return IAM_OK;
 }
+}  // extern "C++"
 
 int iam_model_prefill(iam_model_t m, const int* tokens_host, int n_tokens, int start_pos, float* logits_dev,
                       int* next_token, void* stream) {
-    return run_prefill(m, tokens_host, n_tokens, start_pos, logits_dev, next_token, stream, nullptr);
+    return run_prefill(m, tokens_host, n_tokens, start_pos, logits_dev, next_token, stream, [](int, int) { return (int)IAM_OK; });
 }
 
 int iam_model_score(iam_model_t m, const int* tokens_host, int n_tokens, int start_pos, const int32_t* targets_dev,
@@ -1517,17 +1520,26 @@ int iam_model_set_rope(iam_model_t m, const iam_rope_config* cfg) {
     if (!m) return fail(IAM_ERR_ARG, "iam_model_set_rope: null model");
     std::vector<float> t;
     if (!cfg) {
-        t = rope_table(m->cfg);
+        try {
+            t = rope_table(m->cfg);
+        } catch (const std::bad_alloc&) {
+            return fail(IAM_ERR_NOMEM, "iam_model_set_rope: out of host memory");
+        }
     } else {
         const int rc = rope_check(cfg);
         if (rc) return rc;
         if (cfg->head_dim != m->cfg.head_dim || cfg->rot_dim != cfg->head_dim || cfg->interleaved)
             return fail(IAM_ERR_UNSUPPORTED, "iam_model_set_rope: the model rotates its whole head, in the half layout");
         const int half = cfg->head_dim / 2;
-        std::vector<double> w(half);
+        std::vector<double> w;
         double factor = 1.0;
+        try {
+            w.resize(half);
+            t.resize((size_t)m->cfg.max_ctx * cfg->head_dim);
+        } catch (const std::bad_alloc&) {
+            return fail(IAM_ERR_NOMEM, "iam_model_set_rope: out of host memory");
+        }
         rope_frequencies(*cfg, w.data(), &factor);
-        t.resize((size_t)m->cfg.max_ctx * cfg->head_dim);
         for (int p = 0; p < m->cfg.max_ctx; ++p)
             for (int i = 0; i < half; ++i) {
                 t[((size_t)p * half + i) * 2] = (float)(std::cos(p * w[i]) * factor);

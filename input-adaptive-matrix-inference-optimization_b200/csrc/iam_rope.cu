@@ -222,6 +222,7 @@ extern "C" int iam_rope_apply(iam_rope_t h, int dtype, int n_tokens, const int32
                               const iam_rows* q_out, int n_kv_heads, const iam_rows* k_in, const iam_rows* k_out, void* stream) {
     if (!h) return fail(IAM_ERR_ARG, "rope: null handle");
     if (!dtype_ok(dtype)) return fail(IAM_ERR_ARG, "rope: dtype must be IAM_F32, IAM_F16 or IAM_BF16");
+    if (n_tokens > 1 << 30) return fail(IAM_ERR_ARG, "rope: more than 2^30 tokens");
     if (n_tokens < 0 || n_heads < 0 || n_kv_heads < 0) return fail(IAM_ERR_ARG, "rope: negative count");
     if ((long long)n_heads + n_kv_heads > 65536) return fail(IAM_ERR_ARG, "rope: more than 65536 heads");
     if (n_tokens == 0 || n_heads + n_kv_heads == 0) return IAM_OK;

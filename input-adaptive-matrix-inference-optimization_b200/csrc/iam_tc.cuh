@@ -33,18 +33,6 @@ IAM_DEV bool mbar_try_wait(uint64_t* b, uint32_t parity) {
     return done != 0u;
 }
 
-// One look at the phase, without waiting; one arrival.
-IAM_DEV bool mbar_test(uint64_t* b, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_u32(b)), "r"(parity)
-        : "memory");
-    return done != 0u;
-}
 IAM_DEV void mbar_arrive(uint64_t* b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory"); }
 
 // Waits for the phase of `parity` to complete; false (and the error word set) after ~2 s.

@@ -1,0 +1,67 @@
+"""The 8-bit cache at the ends of its arguments' ranges: windows of any size, queries overwritten by their results, the
+largest tables; limits of the row counts.  Bars and reference are test_kv8_gpu.py's."""
+
+import pytest
+
+from test_kv8_gpu import Batch, close, offsets
+
+# (heads, kv, dim, new rows, type): the kernel for few rows, for some, for many
+KERNELS = [(8, 2, 128, [1, 1, 1], "float16"), (4, 1, 64, [9, 30, 17], "float32"), (8, 1, 128, [60, 33, 64], "bfloat16")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,new,dtype", KERNELS)
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 30])
+def test_the_largest_windows(iam, cuda, heads, kv, dim, new, dtype, window):
+    """Rows before position 0 (the second sequence's) and a window of everything: as without one."""
+    import torch
+    cu, lens = offsets(new), [150, 0, 70]
+    b = Batch(iam, torch, lens, kv, dim, 16, "int8")
+    q = torch.randn(cu[-1], heads, dim, generator=torch.Generator().manual_seed(1)).to(getattr(torch, dtype)).cuda()
+    out, lse = torch.empty_like(q), torch.empty(cu[-1], heads, device="cuda")
+    h = iam.KV8(heads, kv, dim)
+    h.attention(b.cache, q, b.seq_lens, out, cu=torch.tensor(cu, dtype=torch.int32, device="cuda"), max_q=max(new), window=window, lse=lse)
+    h.status()
+    close(out, lse, b.attention_reference(q, cu, 0, torch), torch)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,new,dtype", KERNELS)
+def test_queries_overwritten_by_their_results(iam, cuda, heads, kv, dim, new, dtype):
+    """A context long enough that several CTAs share each tile of rows."""
+    import torch
+    cu, lens = offsets(new), [3000, 40, 900]
+    b = Batch(iam, torch, lens, kv, dim, 64, "e4m3")
+    q = torch.randn(cu[-1], heads, dim, generator=torch.Generator().manual_seed(2)).to(getattr(torch, dtype)).cuda()
+    cud = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    h, out = iam.KV8(heads, kv, dim), torch.empty_like(q)
+    h.attention(b.cache, q, b.seq_lens, out, cu=cud, max_q=max(new))
+    for _ in range(3):
+        x = q.clone()
+        h.attention(b.cache, x, b.seq_lens, x, cu=cud, max_q=max(new))
+        assert torch.equal(x, out)
+    h.status()
+
+
+@pytest.mark.gpu
+def test_tables_and_rows_beyond_the_limits_are_refused(iam, cuda):
+    import torch
+    page = 128
+    b = Batch(iam, torch, [40], 1, 64, page, "int8")
+    h, lens = iam.KV8(1, 1, 64), b.seq_lens
+    q, out = torch.zeros(1, 1, 64, device="cuda"), torch.zeros(1, 1, 64, device="cuda")
+    codes = b.cache.tensors[:4]
+    widest = torch.full((1, 2 ** 26 // page), -1, dtype=torch.int32, device="cuda")
+    widest[:, :b.block_table.shape[1]] = b.block_table
+    h.attention(iam.KV8Cache(*codes, widest), q, lens, out)
+    h.status()
+    too_wide = iam.KV8Cache(*codes, torch.cat((widest, widest[:, -1:]), 1))
+    for call in (lambda: h.attention(too_wide, q, lens, out), lambda: h.append(too_wide, q, q, lens)):
+        with pytest.raises(iam.IamError) as e:
+            call()
+        assert e.value.code == iam.IAM_ERR_UNSUPPORTED
+
+
+def test_row_counts_beyond_the_limits_are_refused(iam):
+    lib = iam.load_library()
+    assert lib.iam_logprobs(None, 0, 2 ** 30 + 1, 8, 8, None, None, None, None, None, 0, None, None, None) == iam.IAM_ERR_ARG
