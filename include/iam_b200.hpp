@@ -184,6 +184,18 @@ class MistralModel {
               "MistralModel::prefill");
         return next;
     }
+    // prefill() that also gives, for each token, the log probability of targets[t] (int32 on the device, the
+    // token whose probability is wanted after it); returns the greedy next token.
+    int score(const int* tokens, int n_tokens, int start_pos, const int* targets_dev, float* logprob_dev, int* rank_dev = nullptr,
+              float* entropy_dev = nullptr) {
+        int next = -1;
+        check(iam_model_score(handle, tokens, n_tokens, start_pos, targets_dev, logprob_dev, entropy_dev, rank_dev, 0, nullptr, nullptr,
+                              &next, gpu->stream),
+              "MistralModel::score");
+        return next;
+    }
+    // Rotary positions scaled for longer contexts (nullptr: the model's own again).
+    void setRope(const iam_rope_config* cfg) { check(iam_model_set_rope(handle, cfg), "MistralModel::setRope"); }
 };
 
 // transformer_layer.hpp:15-122: a decoder layer of a MistralModel (its weights, gains and KV

