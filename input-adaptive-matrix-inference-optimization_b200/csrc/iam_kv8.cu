@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 #include <new>
+#include <type_traits>
 
 #include "iam_kv8.cuh"
 
@@ -10,6 +11,7 @@ namespace iam {
 namespace {
 
 constexpr int kAppendThreads = 256;
+constexpr int kFewRows = 16;     // rows a sequence, on average, up to which a warp does what a block does else
 constexpr int kAppendKeep = 4;  // 16-byte accesses of the new values that a thread keeps between the two passes
 
 template <int FMT>
@@ -79,35 +81,38 @@ struct AppendParams {
 // of that over the sequences before it, so slot w belongs to the last sequence whose base is <= w.
 IAM_DEV int slot_base(int cu, int i, int page_log2) { return (cu >> page_log2) + 2 * i; }
 
-// One block per (touched page, KV head, K or V), the only one that writes that page and head: pass 1
-// finds the largest new value, the block agrees on the scale, pass 2 rounds (and, when the scale grew,
+// NT threads (a block, or one warp of it) per (touched page, KV head, K or V), the only ones that write that page and
+// head: pass 1 finds the largest new value, they agree on the scale, pass 2 rounds (and, when the scale grew,
 // shifts the codes that the page held).  Bound by bytes for prompts (the values are read once and kept
 // in registers up to kAppendKeep accesses a thread), by the chain of dependent loads for single tokens.  15000 tokens
 // of 8 heads of 128, bf16 to e4m3 (91 MB): 27.4 us, 3.3 TB/s (half of it the conversions: with the KV heads of a page
-// apart and single conversions 57); 64 sequences of one token: 7.6 us.
-template <class T, int FMT, bool WIDE>
+// apart and single conversions 57); 64 sequences of one token: 3.0 us.
+template <class T, int FMT, bool WIDE, int NT>
 __global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(AppendParams p) {
     constexpr int VEC = WIDE ? 16 / (int)sizeof(T) : 4;
     using V = Vec<T, VEC>;
-    __shared__ float s_max[kAppendThreads / 32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ float s_max[NT / 32];
+    const int tid = threadIdx.x % NT, lane = tid & 31, warp = tid >> 5;
     // the KV heads of a page side by side, so that blocks at work together read whole token rows
-    const int lots = 2 * p.c.n_kv_heads, slot_no = blockIdx.x / lots, lot = blockIdx.x - slot_no * lots, head = lot >> 1, which = lot & 1;
+    constexpr int ABREAST = kAppendThreads / NT;
+    const int lots = 2 * p.c.n_kv_heads, per_slot = (lots + ABREAST - 1) / ABREAST, slot_no = blockIdx.x / per_slot;
+    const int lot = (blockIdx.x - slot_no * per_slot) * ABREAST + threadIdx.x / NT, head = lot >> 1, which = lot & 1;
     const int page = p.c.page_size, plog = 31 - __clz(page), hd = p.c.head_dim;
     int seq = slot_no, nth = 0;
-    if (p.cu) {  // the sequences whose base is at most this slot
-        int count = 0;
-        for (int i0 = 0; i0 < p.c.n_seqs; i0 += kAppendThreads) {
-            const int i = i0 + tid;
-            const int here = __syncthreads_count(i < p.c.n_seqs && slot_base(p.cu[i], i, plog) <= slot_no);
-            count += here;
-            if (here < kAppendThreads) break;
+    if (p.cu) {  // the last sequence whose base is at most this slot: a probe a thread and round
+        int lo = 0, hi = p.c.n_seqs;
+        while (hi - lo > 1) {
+            const int step = (hi - lo + kAppendThreads - 1) / kAppendThreads, at = lo + threadIdx.x * step;
+            const int below = __syncthreads_count(at < hi && slot_base(p.cu[at], at, plog) <= slot_no);
+            if (below == 0) return;  // (offsets that do not start at 0)
+            hi = min(hi, lo + below * step);
+            lo += (below - 1) * step;
         }
-        seq = count - 1;
-        if (seq < 0) return;
+        seq = lo;
         nth = slot_no - slot_base(p.cu[seq], seq, plog);
         if (nth < 0) return;  // (offsets that do not ascend)
     }
+    if (lot >= lots) return;  // (no barrier of the block behind this with several lots)
     const SeqRows r = seq_rows(p.c, p.cu, p.lens, p.n_rows, seq, p.err);
     const int first = max(r.start, 0);  // tokens before position 0 are skipped
     const long long page_at = (long long)(first / page + nth) * page;  // the page's first token
@@ -126,7 +131,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(AppendPar
     };
 #pragma unroll
     for (int k = 0; k < kAppendKeep; ++k) {
-        const int f = tid + k * kAppendThreads;
+        const int f = tid + k * NT;
         if (f < n_vec) keep[k] = load(f);
     }
     const int id = p.c.block_table[(size_t)seq * p.c.max_pages + index];
@@ -145,8 +150,8 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(AppendPar
     auto each = [&](auto&& f) {
 #pragma unroll
         for (int k = 0; k < kAppendKeep; ++k)
-            if (tid + k * kAppendThreads < n_vec) f(keep[k]);
-        for (int g = tid + kAppendKeep * kAppendThreads; g < n_vec; g += kAppendThreads) f(load(g));
+            if (tid + k * NT < n_vec) f(keep[k]);
+        for (int g = tid + kAppendKeep * NT; g < n_vec; g += NT) f(load(g));
     };
     each([&](const V& v) {
 #pragma unroll
@@ -163,10 +168,12 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(AppendPar
         });
     }
     amax = warp_max(amax);
-    if (lane == 0) s_max[warp] = amax;
-    __syncthreads();
+    if constexpr (NT > 32) {
+        if (lane == 0) s_max[warp] = amax;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, s_max[w]);
+        for (int w = 0; w < NT / 32; ++w) amax = fmaxf(amax, s_max[w]);
+    }
     const float fresh = pow2f(scale_exponent<FMT>(amax));
     const float scale = old > fresh ? old : fresh;
     const float inv = __fdiv_rn(1.0f, scale);
@@ -182,19 +189,23 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(AppendPar
     };
 #pragma unroll
     for (int k = 0; k < kAppendKeep; ++k) {
-        const int f = tid + k * kAppendThreads;
+        const int f = tid + k * NT;
         if (f < n_vec) store(f, keep[k]);
     }
-    for (int f = tid + kAppendKeep * kAppendThreads; f < n_vec; f += kAppendThreads) store(f, load(f));
+    for (int f = tid + kAppendKeep * NT; f < n_vec; f += NT) store(f, load(f));
     if (held > 0 && old < scale) {
         const float shift = __fdiv_rn(old, scale);
-        uint32_t* c4 = reinterpret_cast<uint32_t*>(codes);
-        for (int f = tid; f < held * hd / 4; f += kAppendThreads) {
-            const uint32_t w = c4[f];
-            uint32_t o = 0;
+        uint4* c16 = reinterpret_cast<uint4*>(codes);
+#pragma unroll 4
+        for (int f = tid; f < held * hd / 16; f += NT) {
+            const uint4 w = c16[f];
+            auto moved = [&](uint32_t x) {
+                uint32_t o = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o |= encode<FMT>(decode_code<FMT>((w >> (8 * e)) & 0xffu) * shift) << (8 * e);
-            c4[f] = o;
+                for (int e = 0; e < 4; ++e) o |= encode<FMT>(decode_code<FMT>((x >> (8 * e)) & 0xffu) * shift) << (8 * e);
+                return o;
+            };
+            c16[f] = make_uint4(moved(w.x), moved(w.y), moved(w.z), moved(w.w));
         }
     }
     if (tid == 0) *scale_at = scale;
@@ -308,20 +319,30 @@ extern "C" int iam_kv8_append(iam_kv8_t h, const iam_kv8_cache* cache, int dtype
     if (slots * 2 * cache->n_kv_heads > INT32_MAX) return fail(IAM_ERR_ARG, "kv8: too many sequences");
     AppendParams p{*cache, {*k, *v}, cu_dev, seq_lens_dev, n_rows, h->s.err};
     const bool wide = rows_aligned(*k, elem, 16) && rows_aligned(*v, elem, 16);
-    const dim3 grid((unsigned)(slots * 2 * cache->n_kv_heads));
+    // A block for each page and head, or a warp where there are more of them than blocks run at once and few rows in each
+    // (64 sequences of 1 row: 3.0 us against 7.6, of 16: 5 against 10, of 64: 19 against 16; 512 of 1: 10 against 56; but
+    // 2 of 32, 80 blocks: 5.2 against 3.3).
+    const bool few = n_rows <= kFewRows * (long long)cache->n_seqs && slots * 2 * cache->n_kv_heads > 4LL * h->sms;
+    const int abreast = few ? kAppendThreads / 32 : 1;
+    const dim3 grid((unsigned)(slots * ((2 * cache->n_kv_heads + abreast - 1) / abreast)));
     DeviceGuard g(h->device);
     IAM_CUDA_TRY(g.err);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     rc = with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         // 16-byte reads where every row allows them, else one element at a time
-        if (cache->format == IAM_KV8_INT8) {
-            if (wide) kv8_append_kernel<T, IAM_KV8_INT8, true><<<grid, kAppendThreads, 0, s>>>(p);
-            else kv8_append_kernel<T, IAM_KV8_INT8, false><<<grid, kAppendThreads, 0, s>>>(p);
-        } else {
-            if (wide) kv8_append_kernel<T, IAM_KV8_E4M3, true><<<grid, kAppendThreads, 0, s>>>(p);
-            else kv8_append_kernel<T, IAM_KV8_E4M3, false><<<grid, kAppendThreads, 0, s>>>(p);
-        }
+        auto with_format = [&](auto fmt) {
+            constexpr int FMT = decltype(fmt)::value;
+            if (few) {
+                if (wide) kv8_append_kernel<T, FMT, true, 32><<<grid, kAppendThreads, 0, s>>>(p);
+                else kv8_append_kernel<T, FMT, false, 32><<<grid, kAppendThreads, 0, s>>>(p);
+            } else {
+                if (wide) kv8_append_kernel<T, FMT, true, kAppendThreads><<<grid, kAppendThreads, 0, s>>>(p);
+                else kv8_append_kernel<T, FMT, false, kAppendThreads><<<grid, kAppendThreads, 0, s>>>(p);
+            }
+        };
+        if (cache->format == IAM_KV8_INT8) with_format(std::integral_constant<int, IAM_KV8_INT8>{});
+        else with_format(std::integral_constant<int, IAM_KV8_E4M3>{});
         IAM_CUDA_TRY(cudaGetLastError());
         return (int)IAM_OK;
     });

@@ -3,7 +3,7 @@ largest tables; limits of the row counts.  Bars and reference are test_kv8_gpu.p
 
 import pytest
 
-from test_kv8_gpu import Batch, close, offsets
+from test_kv8_gpu import Batch, close, offsets, reference_append
 
 # (heads, kv, dim, new rows, type): the kernel for few rows, for some, for many
 KERNELS = [(8, 2, 128, [1, 1, 1], "float16"), (4, 1, 64, [9, 30, 17], "float32"), (8, 1, 128, [60, 33, 64], "bfloat16")]
@@ -41,6 +41,38 @@ def test_queries_overwritten_by_their_results(iam, cuda, heads, kv, dim, new, dt
         h.attention(b.cache, x, b.seq_lens, x, cu=cud, max_q=max(new))
         assert torch.equal(x, out)
     h.status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("dtype,fmt,seqs,kv,dim,page,rows", [
+    ("bfloat16", "int8", 120, 3, 128, 16, [1]), ("float32", "e4m3", 300, 5, 64, 32, [0, 1, 2, 7]), ("float16", "int8", 70, 5, 256, 16, [1, 30, 3]),
+    ("bfloat16", "e4m3", 600, 1, 64, 16, [1, 0, 0, 17])])
+def test_append_of_few_rows_to_many_sequences(iam, cuda, dtype, fmt, seqs, kv, dim, page, rows, aligned):
+    """More pages and heads than blocks run at once, heads that leave a part of the last block idle, sequences without
+    rows, one long one among them."""
+    import torch
+    g = torch.Generator().manual_seed(seqs)
+    new = [rows[i % len(rows)] for i in range(seqs)]
+    new[seqs // 2] = 3 * page + 5
+    lens = [n + int(t) for n, t in zip(new, torch.randint(0, 2 * page, (seqs,), generator=g))]
+    cu = offsets(new)
+    b = Batch(iam, torch, lens, kv, dim, page, fmt, seed=3)
+    x = torch.randn(cu[-1] + 2, 2 * kv, dim, generator=g)
+    x[:, ::2] *= 40  # some pages' scales grow, some stay
+    x = x.to(getattr(torch, dtype)).cuda()
+    want = [reference_append(c, s, b.table, r, cu, lens, page, fmt, torch) for c, s, r in
+            ((b.k, b.ks, x[:, :kv]), (b.v, b.vs, x[:, kv:]))]
+    if not aligned:  # rows one element past a 16-byte boundary
+        wide = torch.zeros(x.shape[0], 2 * kv, dim + 1, dtype=x.dtype, device="cuda")
+        wide[:, :, 1:] = x
+        x = wide[:, :, 1:]
+    h = iam.KV8(kv, kv, dim)
+    h.append(b.cache, x[:, :kv], x[:, kv:], b.seq_lens, cu=torch.tensor(cu, dtype=torch.int32, device="cuda"))
+    h.status()
+    for (codes, scales), got, got_s in ((want[0], b.k, b.ks), (want[1], b.v, b.vs)):
+        assert torch.equal(got_s.double(), scales)
+        assert torch.equal(torch.nan_to_num(got.double(), nan=1e9), torch.nan_to_num(codes, nan=1e9))
 
 
 @pytest.mark.gpu
