@@ -116,9 +116,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int PITCH = HD + 4;
     extern __shared__ unsigned char s_raw[];
     // [2] of the first six by tile, of the others by row tile.  No barrier may complete two phases before its waiter has
-    // looked: a row tile's next probabilities can be ready before this one's are waited for, hence two barriers.
+    // looked, nor lag one behind: a row tile's next probabilities can be ready before this one's are waited for, and its sums are
+    // waited for seldom, when the products of the tile before may not be in yet (the other row tile's come first), hence two
+    // barriers each, taken in turn.
     __shared__ __align__(8) uint64_t b_raw_full[2], b_raw_free[2], b_k_ready[2], b_k_free[2], b_v_ready[2], b_v_free[2], b_q_ready[2],
-        b_s_ready[2], b_s_free[2], b_p_ready[2][2], b_o_done[2];
+        b_s_ready[2], b_s_free[2], b_p_ready[2][2], b_o_done[2][2];
     __shared__ float4 s_info[kInfo][kGroups];  // key scale, value scale, 1 if the page is one of the cache's, log2 of the value scale
     __shared__ uint32_t s_tmem;
     __shared__ int s_last;
@@ -135,7 +137,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&b_s_free[i], 4);
             mbar_init(&b_p_ready[i][0], 4);
             mbar_init(&b_p_ready[i][1], 4);
-            mbar_init(&b_o_done[i], 1);
+            mbar_init(&b_o_done[i][0], 1);
+            mbar_init(&b_o_done[i][1], 1);
             mbar_init(&b_k_ready[i], 4);
             mbar_init(&b_k_free[i], 1);
             mbar_init(&b_v_ready[i], 4);
@@ -267,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int k = 0; k < kTile / 16; ++k)
                         tc_mma_ts(tm_o(i), tm_p(i, place) + 8 * k, vals + (uint64_t)(2 * k), kDescO, !first || k > 0);
-                    tc_commit(&b_o_done[i]);
+                    tc_commit(&b_o_done[i][place]);
                 }
             };
             auto commit = [&](uint64_t* b) {
@@ -477,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         l *= fm;
                         m = raise ? mx : m;
                         if (j > 0) {
-                            wait(&b_o_done[i], ni - 1);  // the products of the tile before are in
+                            wait(&b_o_done[i][(ni - 1) & 1], (ni - 1) >> 1);  // the products of the tile before are in
                             tc_fence_after();
 #pragma unroll 1
                             for (int c = 0; c < HD / 16; ++c) {
@@ -537,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             constexpr int PART = kRows * PITCH;
             float* part = p.s.part + (size_t)(2 * blockIdx.x + ((int)blockIdx.x == cta0 ? 1 : 0)) * PART;
             if (tile_there) {
-                wait(&b_o_done[i], ni - 1);
+                wait(&b_o_done[i][(ni - 1) & 1], (ni - 1) >> 1);
                 tc_fence_after();
                 const float scale = unit * (1.0f / (1 << kLiftLog));
 #pragma unroll

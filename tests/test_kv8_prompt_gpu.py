@@ -96,3 +96,27 @@ def test_prompt_page_out_of_range(iam, cuda):
     want = b.attention_reference(q[:200], [0, 200, 200], 0, torch)
     close(out[:200], None, want, torch)
     assert out.isfinite().all()
+
+
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("heads,kv,dim,page,fmt,lens,new,window", [
+    (8, 2, 128, 64, "int8", [300], [200], 0), (4, 1, 128, 16, "e4m3", [700, 330], [150, 330], 0), (16, 2, 64, 32, "int8", [500, 400], [90, 160], 130),
+    (32, 8, 128, 64, "e4m3", [900], [256], 0)])
+def test_prompt_attention_repeats_to_the_bit(iam, cuda, heads, kv, dim, page, fmt, lens, new, window):
+    """Row tiles with unequal work (masked tiles in one and not in the other), many times over: a tile's sums are read when
+    all of its products are in, however far the other row tile is behind."""
+    import torch
+    cu = offsets(new)
+    b = Batch(iam, torch, lens, kv, dim, page, fmt, seed=5)
+    q = torch.randn(cu[-1], heads, dim, generator=torch.Generator().manual_seed(3)).half().cuda()
+    h, out, first = iam.KV8(heads, kv, dim), torch.empty_like(q), None
+    cud = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    off = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(3000):
+        h.attention(b.cache, q, b.seq_lens, out, cu=cud, max_q=max(new), window=window)
+        if first is None:
+            first = out.clone()
+            close(first, None, b.attention_reference(q, cu, window, torch), torch)
+        off += (out != first).any()
+    h.status()
+    assert int(off) == 0
