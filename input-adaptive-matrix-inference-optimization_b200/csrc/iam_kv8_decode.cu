@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
     auto sharers = [&](const Items& it) {
         return min(1 + (int)((long long)it.nt * (grid - n_items) / n_groups), (it.nt + kMinGroups - 1) / kMinGroups);
     };
-    const int total = (int)line, ctas = min(grid, (int)min((n_groups + kMinGroups - 1) / kMinGroups, (long long)grid));
+    const int total = (int)line, ctas = (int)min((long long)grid, max(n_items, (n_groups + kMinGroups - 1) / kMinGroups));
     if (!few && (int)blockIdx.x >= ctas) return;
     const Cut cut{total / ctas, total % ctas};
     const int u0 = few ? (int)blockIdx.x : cut.first(blockIdx.x), u1 = few ? u0 + 1 : cut.first(blockIdx.x + 1);

@@ -163,7 +163,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int items = plan.items();
     const int per_head = plan.unit()[items];
     const long long total = (long long)per_head * kvh;
-    const long long ctas = min((long long)gridDim.x, (total + kMinUnits - 1) / kMinUnits);
+    const int run = min(kMinUnits, per_head / max(1, items));  // (short contexts: a row tile a CTA)
+    const long long ctas = min((long long)gridDim.x, (total + run - 1) / max(1, run));
     const bool idle = (long long)blockIdx.x >= ctas;
     const long long u0 = idle ? 0 : total * blockIdx.x / ctas, u1 = idle ? 0 : total * (blockIdx.x + 1) / ctas;
 

@@ -42,7 +42,8 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(Kv8Attn p) {
     const int per_head = plan.unit()[items];
     const long long total = (long long)per_head * kvh;
     if (total == 0) return;
-    const long long ctas = min((long long)gridDim.x, (total + kMinUnits - 1) / kMinUnits);
+    const int run = min(kMinUnits, per_head / max(1, items));  // (short contexts: a row tile a CTA)
+    const long long ctas = min((long long)gridDim.x, (total + run - 1) / max(1, run));
     if (blockIdx.x >= ctas) return;
     const long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
     int item = find_item(plan, items, (int)(u0 % per_head));
