@@ -82,9 +82,13 @@ constexpr float kLn2 = 0.69314718055994530942f;
 
 // A row's result from its running maximum (log2 domain), sum and value sums.
 template <class T>
+IAM_DEV T result(float o, float l) {
+    return from_f32<T>(l > 0.0f || l != l ? __fdiv_rn(o, l) : 0.0f);
+}
+template <class T>
 IAM_DEV void store_result(const Kv8Attn& p, size_t row, int head, int d, float o, float l) {
     T* out = static_cast<T*>(p.out.data) + row * p.out.token_stride + head * p.out.head_stride;
-    out[d] = from_f32<T>(l > 0.0f || l != l ? __fdiv_rn(o, l) : 0.0f);
+    out[d] = result<T>(o, l);
 }
 IAM_DEV void store_lse(const Kv8Attn& p, size_t row, int head, float m, float l) {
     if (p.lse) p.lse[row * p.n_heads + head] = l > 0.0f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY;

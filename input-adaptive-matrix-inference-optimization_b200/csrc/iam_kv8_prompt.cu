@@ -13,7 +13,8 @@
 //   13           the copies (TMA, 16 rows a box, so any page size)
 // 128 x 128 rows and tokens cost the tensor cores 512 cycles for S and as many for P V (head_dim 128), and their 16384
 // powers cost the special-function units 1024: the two are level, and neither can wait for the other.  2048 rows on 8192
-// earlier tokens (32 heads of 128 over 8): 600 us, 515 TFLOP/s.  Bound by the softmax's chain from one tile's scores to
+// earlier tokens (32 heads of 128 over 8): 494 us, 625 TFLOP/s
+// (queries and results moved 2 bytes at a time: 606).  Bound by the softmax's chain from one tile's scores to
 // its probabilities, some 3200 cycles for 256 x 64; the mma.sync kernel for rows took 2001.
 #include <algorithm>
 #include <atomic>
@@ -398,18 +399,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             float rf = 0.0f;
             if (tile_there) {  // this thread's query, shifted into fp16's range
                 const T* src = have ? static_cast<const T*>(p.q.data) + q_row * p.q.token_stride + q_head * p.q.head_stride : nullptr;
+                // (16 bytes at a time where the row allows it: as many trips less for the start of a piece)
+                const bool wide = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+                auto eight = [&](int c) { return wide ? load_vec<true, T, 8>(src + c * 8) : load_vec<false, T, 8>(src + c * 8); };
                 float amax = 0.0f;
                 if (have)
 #pragma unroll 8
-                    for (int d = 0; d < HD; ++d) amax = fmaxf(amax, fabsf(to_f32(src[d])));
+                    for (int c = 0; c < HD / 8; ++c) {
+                        const Vec<T, 8> x = eight(c);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(to_f32(x.v[e])));
+                    }
                 const int sh = query_shift(amax);
                 const float up = pow2f(sh);
                 rf = pow2f(-sh) * p.scale_log2;
 #pragma unroll 2
                 for (int c = 0; c < HD / 8; ++c) {
                     float f[8];
+                    Vec<T, 8> x;
+                    if (have) x = eight(c);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] = have ? to_f32(src[c * 8 + e]) * up : 0.0f;
+                    for (int e = 0; e < 8; ++e) f[e] = have ? to_f32(x.v[e]) * up : 0.0f;
                     *reinterpret_cast<uint4*>(smem + M::q + i * M::kQBytes + (c >> 3) * (kQ * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
                         make_uint4(cvt_h2(f[0], f[1]), cvt_h2(f[2], f[3]), cvt_h2(f[4], f[5]), cvt_h2(f[6], f[7]));
                 }
@@ -550,6 +560,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_ld32(to + 32 * c, x);
                     tmem_ld_wait(x);
                     if (!have) continue;
+                    T* const out = static_cast<T*>(p.out.data) + q_row * p.out.token_stride + q_head * p.out.head_stride + 32 * c;
+                    if (complete && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            Vec<T, 8> v;
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) v.v[k] = result<T>(__uint_as_float(x[e + k]) * scale, l);
+                            store_vec<true>(out + e, v);
+                        }
+                        continue;
+                    }
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
                         const float4 v = make_float4(__uint_as_float(x[e]) * scale, __uint_as_float(x[e + 1]) * scale,
