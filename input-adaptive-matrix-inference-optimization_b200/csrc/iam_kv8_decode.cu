@@ -23,6 +23,9 @@ namespace {
 
 constexpr int kMinGroups = 8;  // groups of tokens of a CTA at least, where a context is shared
 constexpr int kItemCost = 24;  // what opening and joining a piece of a context costs, in groups
+// Probabilities (at most 1) are lifted by this before they are rounded to fp16, whose smallest step is 2^-24: a weight of 2^-28
+// still has all of its 11 bits, and what is lost of smaller ones is 2^-39 of the largest value a token.
+constexpr float kLift = 16384.0f;
 
 // Warps of a CTA (one CTA an SM; as many as have the registers they need) and groups of 16 tokens in each warp's
 // ring: 128 to 144 KB of codes on their way.
@@ -86,7 +89,8 @@ IAM_DEV uint32_t transpose8(uint32_t v) {
 }
 
 // T: query and output type; TERMS 2 (fp32): columns 0..3 of the tile hold the rows' high fp16 terms and
-// 4..7 the low ones (and so for the probabilities), which carries 22 bits of both through fp16 products.
+// 4..7 the low ones (and so for the probabilities), which carries 22 bits of both through fp16 products (of a probability, down
+// to 2^-17 of its warp's maximum, where the low term meets fp16's smallest step).
 // Each warp streams its own groups of tokens through its own ring in shared memory: TMA fetches a group's keys and
 // values (16 rows each, swizzled so that the reads below meet no bank twice) as soon as the warp has taken an
 // earlier group out of that place, into the next piece of context already; the warps wait for one another only
@@ -438,6 +442,8 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
                 sc[2 + h] = ex2(s1 - ref);
                 l[h] = fmaf(l[h], rescale[h], sc[h] + sc[2 + h]);  // this lane's tokens only
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[e] *= kLift;  // (the sums l are of the weights as they are)
             if (TERMS == 2 && tig >= 2)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sc[e] = split_lo(sc[e]);
@@ -505,7 +511,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
             for (int e = 0; e < 4; ++e) {
                 const int c = mt >> 1;
                 const int dim = (VW == 2 ? 8 * g + 4 * c : (c >> 2) * 128 + 16 * g + 4 * (c & 3)) + 2 * (mt & 1) + (e >> 1);
-                s_o[warp][2 * tig + (e & 1)][dim] = o[mt][e] * unit;
+                s_o[warp][2 * tig + (e & 1)][dim] = o[mt][e] * (1.0f / kLift) * unit;
             }
         __syncthreads();
         // the next piece's queries are on their way while this one's results are joined
