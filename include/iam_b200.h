@@ -269,7 +269,8 @@ int iam_kv8_append(iam_kv8_t h, const iam_kv8_cache* cache, int dtype, int n_row
  * (p - window, p] (window 0: all up to p); query head j reads KV head j / (n_heads / n_kv_heads).
  * scale 0: 1/sqrt(head_dim).  out has q's dtype; lse_dev (may be NULL) [n_rows][n_heads] fp32
  * receives the natural logarithm of the sum of exponentials.  A row that sees nothing (a position
- * below 0) gives 0 and -inf.  out may be q itself (with its strides).  At most 65536 tiles of 64 rows (n_rows * n_heads /
+ * below 0) gives 0 and -inf.  Scores, maxima and sums are in fp32; the probabilities that multiply the values are
+ * rounded to fp16 (11 bits) with 16-bit queries and carry 22 bits with fp32 ones.  out may be q itself (with its strides).  At most 65536 tiles of 64 rows (n_rows * n_heads /
  * n_kv_heads / 64 + n_seqs).  max_q: a bound on one sequence's rows, if known (0: n_rows); it
  * chooses the kernel and never the result's meaning.  What stands in a page behind the sequence's
  * last token has no influence. */
