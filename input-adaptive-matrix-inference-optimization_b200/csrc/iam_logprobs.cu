@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(LogprobParam
         mbar_expect_tx(&s_full, bytes);
         if (bytes) bulk_load(s_chunk + (size_t)(a - c0) * 16, w.x - w.lead + (size_t)a * VEC, bytes, &s_full);
     };
+    if (C > 1) cluster.barrier_arrive();
     if (tid == 0) {
         mbar_init(&s_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -150,6 +151,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(LogprobParam
     __syncthreads();
     int row = blockIdx.x / C;
     if (tid == 0 && row < n_rows) fetch(where(row), where(row).v0);
+    // The first CTA's shared memory takes the others' parts only once that CTA runs; the first chunk is on its way meanwhile.
+    if (C > 1) {
+        __syncwarp();
+        cluster.barrier_wait();
+    }
     uint32_t phase = 0;
     for (int turn = 0; row < n_rows; row += step, turn ^= 1) {  // (every CTA of a cluster makes the same turns)
         const Where w = where(row);

@@ -172,3 +172,32 @@ def test_refused_calls(iam, cuda):
         with pytest.raises(iam.IamError) as e:
             iam.logprobs(**dict(dict(logits=x, targets=t), **change))
         assert e.value.code == iam.IAM_ERR_ARG
+
+
+def test_few_rows_on_a_busy_device(iam, cuda):
+    """Rows shared by a cluster's CTAs, whose parts meet in the first one's memory: many short calls on several streams at once,
+    beside products that keep most SMs busy, so that the CTAs of a cluster start at different times."""
+    import torch
+    g = torch.Generator("cuda").manual_seed(11)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    jobs = []
+    for i, (n, vocab, k) in enumerate([(1, 131071, 64), (2, 32000, 5), (3, 70001, 40), (1, 8209, 20)]):
+        x = torch.randn(n, vocab, generator=g, device="cuda") * 3
+        targets = torch.randint(0, vocab, (n,), generator=g, device="cuda", dtype=torch.int32)
+        first = call(iam, x, targets, k, torch)
+        compare(first, reference(x, targets, k, torch), x, k, torch)
+        jobs.append((x, targets, k, first, {name: t.clone() for name, t in first.items()}, torch.zeros((), dtype=torch.int64, device="cuda")))
+    a = torch.randn(2048, 2048, device="cuda")
+    busy = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(200):
+        with torch.cuda.stream(busy):
+            a = (a @ a).clamp(-1, 1)
+        for s, (x, targets, k, first, out, off) in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                iam.logprobs(x, targets, **out)
+                for name in out:
+                    off += (out[name] != first[name]).any()
+                    out[name].zero_()
+    torch.cuda.synchronize()
+    assert all(int(job[-1]) == 0 for job in jobs)
