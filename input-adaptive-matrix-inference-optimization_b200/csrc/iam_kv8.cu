@@ -173,6 +173,8 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(AppendPar
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < NT / 32; ++w) amax = fmaxf(amax, s_max[w]);
+    } else {
+        __syncwarp();  // every lane has read the old scale before one overwrites it
     }
     const float fresh = pow2f(scale_exponent<FMT>(amax));
     const float scale = old > fresh ? old : fresh;

@@ -3,7 +3,7 @@ largest tables; limits of the row counts.  Bars and reference are test_kv8_gpu.p
 
 import pytest
 
-from test_kv8_gpu import Batch, close, offsets, reference_append
+from test_kv8_gpu import Batch, close, nearest, offsets, reference_append
 
 # (heads, kv, dim, new rows, type): the kernel for few rows, for some, for many
 KERNELS = [(8, 2, 128, [1, 1, 1], "float16"), (4, 1, 64, [9, 30, 17], "float32"), (8, 1, 128, [60, 33, 64], "bfloat16")]
@@ -73,6 +73,44 @@ def test_append_of_few_rows_to_many_sequences(iam, cuda, dtype, fmt, seqs, kv, d
     for (codes, scales), got, got_s in ((want[0], b.k, b.ks), (want[1], b.v, b.vs)):
         assert torch.equal(got_s.double(), scales)
         assert torch.equal(torch.nan_to_num(got.double(), nan=1e9), torch.nan_to_num(codes, nan=1e9))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,fmt", [("float32", "int8"), ("bfloat16", "e4m3")])
+def test_growing_scales_in_many_sequences(iam, cuda, dtype, fmt):
+    """A warp a page and head: each appended token is larger than all before it, so that every page shifts what it holds
+    while its scale is replaced, 40 tokens in a row for 200 sequences."""
+    import torch
+    seqs, kv, dim, page = 200, 2, 128, 32
+    b = Batch(iam, torch, [40] * seqs, kv, dim, page, fmt, seed=6)
+    codes, scales = [b.k.clone(), b.v.clone()], [b.ks.clone(), b.vs.clone()]
+    h = iam.KV8(kv, kv, dim)
+    g = torch.Generator().manual_seed(8)
+    for t in range(40):
+        x = (torch.randn(seqs, 2 * kv, dim, generator=g) * 1.6 ** t).to(getattr(torch, dtype)).cuda()
+        lens = torch.full((seqs,), t + 1, dtype=torch.int32, device="cuda")
+        h.append(b.cache, x[:, :kv], x[:, kv:], lens)
+        if t in (7, 31, 32, 39):
+            h.status()
+        for i, part in enumerate((x[:, :kv], x[:, kv:])):
+            # the definition for one token of each sequence, all at once (powers of two: exact)
+            at = torch.tensor([r[t // page] for r in b.table], device="cuda")
+            row, old = t % page, scales[i][at].double()
+            amax = part.double().abs().amax(-1)
+            need = torch.exp2(torch.ceil(torch.log2(amax / (127.0 if fmt == "int8" else 448.0))))
+            now = torch.maximum(old, need) if row else need
+            held = codes[i][at].double()
+            held[:, :, :row] = nearest(held[:, :, :row] * (old / now)[..., None, None], fmt, torch)
+            held[:, :, row] = nearest(part.double() / now[..., None], fmt, torch)
+            codes[i][at] = held.float().to(codes[i].dtype)
+            scales[i][at] = now.float()
+    for got, got_s, want, want_s in ((b.k, b.ks, codes[0], scales[0]), (b.v, b.vs, codes[1], scales[1])):
+        used = torch.tensor(b.table, device="cuda").flatten()
+        assert torch.equal(got_s[used], want_s[used])
+        last = torch.tensor([r[1] for r in b.table], device="cuda")
+        first = torch.tensor([r[0] for r in b.table], device="cuda")
+        assert torch.equal(got[first].float(), want[first].float())
+        assert torch.equal(got[last].float()[:, :, :40 - page], want[last].float()[:, :, :40 - page])
 
 
 @pytest.mark.gpu
