@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             atomicOr(p.s.err, kKv8ErrWait);
             dead = true;
         }
+        __syncwarp();  // (lanes may leave the wait one by one, and what follows it takes the whole warp together)
     };
     auto give = [&](uint64_t* b) {  // one arrival for this warp
         __syncwarp();
@@ -482,6 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         mx = fmaxf(mx, gm == -INFINITY ? gm : gm * f);
                     }
+                    if constexpr (!PLAIN) __syncwarp();  // (the masks may part the warp; nothing behind them does)
                     // The reference follows the maximum with a lag: powers of up to 2^kLag are as exact, and O is
                     // rarely rewritten.  O is in units of the largest value scale so far.
                     const bool raise = mx > m + kLag || (m == -INFINITY && mx > -INFINITY);
@@ -554,34 +556,39 @@ __global__ void __launch_bounds__(kThreads, 1)
                 wait(&b_o_done[i][(ni - 1) & 1], (ni - 1) >> 1);
                 tc_fence_after();
                 const float scale = unit * (1.0f / (1 << kLiftLog));
+                // (decided once for all rows, so that the warp stays together)
+                const bool wide = ((reinterpret_cast<uintptr_t>(p.out.data) | (uintptr_t)(p.out.token_stride * (long long)sizeof(T)) |
+                                    (uintptr_t)(p.out.head_stride * (long long)sizeof(T))) & 15) == 0;
 #pragma unroll
                 for (int c = 0; c < HD / 32; ++c) {
                     uint32_t x[32];
+                    __syncwarp();  // a row tile's last rows may be none: the load takes all lanes together
                     tmem_ld32(to + 32 * c, x);
                     tmem_ld_wait(x);
-                    if (!have) continue;
-                    T* const out = static_cast<T*>(p.out.data) + q_row * p.out.token_stride + q_head * p.out.head_stride + 32 * c;
-                    if (complete && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+                    if (have) {
+                        if (complete && wide) {
+                            T* const out = static_cast<T*>(p.out.data) + q_row * p.out.token_stride + q_head * p.out.head_stride + 32 * c;
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            Vec<T, 8> v;
+                            for (int e = 0; e < 32; e += 8) {
+                                Vec<T, 8> v;
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) v.v[k] = result<T>(__uint_as_float(x[e + k]) * scale, l);
-                            store_vec<true>(out + e, v);
-                        }
-                        continue;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 v = make_float4(__uint_as_float(x[e]) * scale, __uint_as_float(x[e + 1]) * scale,
-                                                     __uint_as_float(x[e + 2]) * scale, __uint_as_float(x[e + 3]) * scale);
-                        if (complete) {
-                            store_result<T>(p, q_row, q_head, 32 * c + e, v.x, l);
-                            store_result<T>(p, q_row, q_head, 32 * c + e + 1, v.y, l);
-                            store_result<T>(p, q_row, q_head, 32 * c + e + 2, v.z, l);
-                            store_result<T>(p, q_row, q_head, 32 * c + e + 3, v.w, l);
+                                for (int k = 0; k < 8; ++k) v.v[k] = result<T>(__uint_as_float(x[e + k]) * scale, l);
+                                store_vec<true>(out + e, v);
+                            }
                         } else {
-                            __stcg(reinterpret_cast<float4*>(part + mine * PITCH + 32 * c + e), v);
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) {
+                                const float4 v = make_float4(__uint_as_float(x[e]) * scale, __uint_as_float(x[e + 1]) * scale,
+                                                             __uint_as_float(x[e + 2]) * scale, __uint_as_float(x[e + 3]) * scale);
+                                if (complete) {
+                                    store_result<T>(p, q_row, q_head, 32 * c + e, v.x, l);
+                                    store_result<T>(p, q_row, q_head, 32 * c + e + 1, v.y, l);
+                                    store_result<T>(p, q_row, q_head, 32 * c + e + 2, v.z, l);
+                                    store_result<T>(p, q_row, q_head, 32 * c + e + 3, v.w, l);
+                                } else {
+                                    __stcg(reinterpret_cast<float4*>(part + mine * PITCH + 32 * c + e), v);
+                                }
+                            }
                         }
                     }
                 }

@@ -120,3 +120,24 @@ def test_prompt_attention_repeats_to_the_bit(iam, cuda, heads, kv, dim, page, fm
         off += (out != first).any()
     h.status()
     assert int(off) == 0
+
+
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("gap", [0, 8, 3])
+@pytest.mark.parametrize("heads,kv,dim,new", [(3, 1, 128, [43, 61, 90, 1]), (5, 1, 64, [57, 103, 2]), (1, 1, 128, [129, 257, 300])])
+def test_row_tiles_that_end_inside_a_warp(iam, cuda, heads, kv, dim, new, gap):
+    """Lanes with and without a row beside each other, in every warp of a tile; results at 16-byte boundaries, off them, and in
+    some rows on and in others off them (a gap of 3 elements between the heads)."""
+    import torch
+    cu, lens = offsets(new), [n + 70 * i for i, n in enumerate(new)]
+    b = Batch(iam, torch, lens, kv, dim, 16, "int8", seed=9)
+    q = torch.randn(cu[-1], heads, dim, generator=torch.Generator().manual_seed(4)).half().cuda()
+    room = torch.full((cu[-1] + 1, heads, dim + gap), 5.0, dtype=torch.half, device="cuda")
+    out, lse = room[:cu[-1], :, gap:], torch.empty(cu[-1], heads, device="cuda")
+    h = iam.KV8(heads, kv, dim)
+    cud = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    h.attention(b.cache, q, b.seq_lens, out, cu=cud, lse=lse)
+    h.status()
+    close(out, lse, b.attention_reference(q, cu, 0, torch), torch)
+    assert (room[cu[-1]:] == 5.0).all() and (room[:, :, :gap] == 5.0).all()
+    h.close()

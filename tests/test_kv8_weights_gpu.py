@@ -69,3 +69,12 @@ def test_small_weights_in_decoding(iam, cuda, heads, kv, dim, seqs, dtype, fmt, 
     """Enough sequences that each is read by few warps (several thousand tokens a warp), and one that many CTAs share."""
     import torch
     run(iam, torch, heads, kv, dim, seqs, [6001, 4097], 1, dtype, fmt, c, dtype == "float32", 2.0 ** 14, 1)
+
+
+@pytest.mark.parametrize("c", [12.06, 14.82, 17.95])
+@pytest.mark.parametrize("heads,kv,dim,seqs,new,dtype,two_terms,lift", [
+    (2, 1, 128, 3, 70, "float32", True, 2.0 ** 12), (2, 1, 256, 2, 64, "bfloat16", False, 2.0 ** 12), (2, 2, 64, 1, 300, "float16", False, 2.0 ** 7),
+    (4, 1, 128, 2, 130, "bfloat16", False, 2.0 ** 7)])
+def test_small_weights_in_prompts(iam, cuda, heads, kv, dim, seqs, new, dtype, two_terms, lift, c):
+    import torch
+    run(iam, torch, heads, kv, dim, seqs, [4000], new, dtype, "int8", c, two_terms, lift, new)
