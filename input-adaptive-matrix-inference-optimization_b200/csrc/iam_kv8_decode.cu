@@ -369,6 +369,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
             const unsigned char* box_k = mine_ring + st * S::kStage;
             const unsigned char* box_v = box_k + S::kHalves * S::kBox;
             if (!mbar_wait(&s_full[warp][st], (n_used / S::kStages) & 1, nullptr)) atomicOr(p.s.err, kKv8ErrWait);
+            __syncwarp();  // (lanes may leave the wait one by one; the matrix instructions take the warp together)
             const float4 group = s_group[warp][st];
             const float ks_now = group.x, vs_now = group.y;
             const bool bad = __float_as_int(group.z) < 0;
@@ -411,7 +412,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
             }
             ++n_used;
             __syncwarp();
-            issue();
+            issue();  // (what parts the warp here and in the masks meets again at the maxima's shuffles)
             if (t + kKv8Group > r.cap || bad) {  // what stands behind the last token has no part in the sums
 #pragma unroll
                 for (int j = 0; j < 4; ++j)

@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(Kv8Attn p) {
             }
             __syncthreads();
             if (i + 1 < n_tiles) issue(i + 1);
+            __syncwarp();  // (pages may part the warp, and the matrix instructions take it together)
 
             float sc[NT][4];
 #pragma unroll
@@ -244,6 +245,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(Kv8Attn p) {
                 }
             }
             const float vf = vmax * (1.0f / 4096.0f);
+            __syncwarp();
 #pragma unroll
             for (int n2 = 0; n2 < HD / 16; ++n2) {
                 float acc[2][4];

@@ -44,6 +44,27 @@ def test_queries_overwritten_by_their_results(iam, cuda, heads, kv, dim, new, dt
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("window", [0, 5, 17])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(4, 2, 64, "float32"), (4, 1, 128, "bfloat16"), (2, 1, 256, "float16"), (24, 1, 64, "float16"),
+                                                (30, 1, 128, "float32")])
+def test_lengths_around_a_group_of_tokens(iam, cuda, heads, kv, dim, dtype, fmt, window):
+    """Sequences of 1 to 50 tokens with up to three rows each (the kernel for few rows and the one for some): the last token, the
+    rows' own limits and the window's start at every place of a group of 16, where masks part the lanes."""
+    import torch
+    lens = list(range(1, 51))
+    new = [1 + i % 3 for i in lens]
+    cu = offsets(new)
+    b = Batch(iam, torch, lens, kv, dim, 16, fmt, seed=12)
+    q = torch.randn(cu[-1], heads, dim, generator=torch.Generator().manual_seed(3)).to(getattr(torch, dtype)).cuda()
+    out, lse = torch.empty_like(q), torch.empty(cu[-1], heads, device="cuda")
+    h = iam.KV8(heads, kv, dim)
+    h.attention(b.cache, q, b.seq_lens, out, cu=torch.tensor(cu, dtype=torch.int32, device="cuda"), max_q=3, window=window, lse=lse)
+    h.status()
+    close(out, lse, b.attention_reference(q, cu, window, torch), torch)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("aligned", [True, False])
 @pytest.mark.parametrize("dtype,fmt,seqs,kv,dim,page,rows", [
     ("bfloat16", "int8", 120, 3, 128, 16, [1]), ("float32", "e4m3", 300, 5, 64, 32, [0, 1, 2, 7]), ("float16", "int8", 70, 5, 256, 16, [1, 30, 3]),
