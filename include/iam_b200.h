@@ -273,7 +273,8 @@ int iam_kv8_append(iam_kv8_t h, const iam_kv8_cache* cache, int dtype, int n_row
  * rounded to fp16 (11 bits) with 16-bit queries and carry 22 bits with fp32 ones.  out may be q itself (with its strides).  At most 65536 tiles of 64 rows (n_rows * n_heads /
  * n_kv_heads / 64 + n_seqs).  max_q: a bound on one sequence's rows, if known (0: n_rows); it
  * chooses the kernel and never the result's meaning.  What stands in a page behind the sequence's
- * last token has no influence. */
+ * last token, or before the window of its first row, has no influence, and pages that lie wholly before that window are not
+ * looked up (their table entries may name any page or none). */
 int iam_kv8_attention(iam_kv8_t h, const iam_kv8_cache* cache, int dtype, int n_rows, int max_q, const iam_rows* q,
                       const int32_t* cu_dev, const int32_t* seq_lens_dev, float scale, int window, const iam_rows* out,
                       float* lse_dev, void* stream);

@@ -413,12 +413,15 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
             ++n_used;
             __syncwarp();
             issue();  // (what parts the warp here and in the masks meets again at the maxima's shuffles)
-            if (t + kKv8Group > r.cap || bad) {  // what stands behind the last token has no part in the sums
+            // what stands behind the last token or before the window has no part in the sums
+            if (t + kKv8Group > r.cap || bad || (p.window > 0 && t <= pos_lo - p.window)) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (bad || t + token(2 * tig + (j & 1)) + (j >> 1) * 8 >= r.cap)
+                for (int j = 0; j < 4; ++j) {
+                    const int at = t + token(2 * tig + (j & 1)) + (j >> 1) * 8;
+                    if (bad || at >= r.cap || (p.window > 0 && at <= pos_lo - p.window))
 #pragma unroll
                         for (int c = 0; c < VW; ++c) vq[j][c] = 0u;
+                }
             }
             if (TERMS == 2)
 #pragma unroll

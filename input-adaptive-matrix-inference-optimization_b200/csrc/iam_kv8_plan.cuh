@@ -23,7 +23,8 @@ struct Plan {
 };
 
 struct RowItem {
-    int lo, nt, pos_lo, pos_hi, n_rows;  // first token read (a multiple of TILE), units, first and last position
+    int lo, nt, pos_lo, pos_hi, n_rows;  // first token of the first unit (a multiple of TILE), units, first and last position
+    int first;                           // first token that a row sees: pages wholly before it are not looked up
 };
 
 template <int ROWS, int TILE>
@@ -32,7 +33,8 @@ IAM_DEV RowItem item_of(const Kv8Attn& p, const SeqRows& r, int rtile) {
     it.n_rows = min(ROWS, r.n * p.gq - rtile * ROWS);
     it.pos_lo = r.start + rtile * ROWS / p.gq;
     it.pos_hi = r.start + (rtile * ROWS + it.n_rows - 1) / p.gq;
-    it.lo = p.window > 0 ? max(0, it.pos_lo - p.window + 1) & ~(TILE - 1) : 0;
+    it.first = p.window > 0 ? max(0, it.pos_lo - p.window + 1) : 0;
+    it.lo = it.first & ~(TILE - 1);
     const int hi = min(it.pos_hi + 1, r.cap);
     it.nt = max(1, (hi - it.lo + TILE - 1) / TILE);
     return it;

@@ -214,9 +214,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int n = 0; u < u1; close()) {
             open();
             const int32_t* table = p.c.block_table + (size_t)w.seq * p.c.max_pages;
+            const int from = w.it.first & ~(kKv8Group - 1);  // (pages wholly before the window may be anyone's)
             auto page_of = [&](int j) {
                 const int t = w.t_first + j * kTile + lane * kKv8Group;
-                return lane < kGroups && j < w.n_tiles && t < w.r.cap ? __ldg(table + (t >> plog)) : -1;
+                return lane < kGroups && j < w.n_tiles && t < w.r.cap && t >= from ? __ldg(table + (t >> plog)) : -1;
             };
             int id = page_of(0);
             for (int j = 0; j < w.n_tiles; ++j, ++n) {
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int id_next = page_of(j + 1);
                 wait(&b_raw_free[st], (n >> 1) + 1);
                 if (lane < kGroups) {
-                    if (t < w.r.cap && (id < 0 || id >= p.c.n_pages)) {
+                    if (t < w.r.cap && t >= from && (id < 0 || id >= p.c.n_pages)) {
                         atomicOr(p.s.err, kKv8ErrRange);
                         id = -1;
                     }
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // values: 4 dims of 8 tokens to 4 rows of 16 bytes; lanes take the tokens in turn, so that neither
                 // reads nor stores meet a bank twice
                 constexpr int WORDS = HD / 4;
-                const bool ends = t0 + kTile > w.r.cap;
+                const bool ends = t0 + kTile > w.r.cap || t0 < w.it.first;
                 unsigned ok = 0;
 #pragma unroll
                 for (int k = 0; k < kGroups; ++k) ok |= s_info[n % kInfo][k].z != 0.0f ? 1u << k : 0u;
@@ -361,10 +362,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint32_t v[8];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const uint32_t*>(raw_v + (t8 * 8 + k) * HD + word * 4);
-                    if (ends || ok != (1u << kGroups) - 1u)  // what stands behind the last token has no part in the sums
+                    if (ends || ok != (1u << kGroups) - 1u)  // what stands behind the last token or before the window has no part in the sums
 #pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            if (t0 + t8 * 8 + k >= w.r.cap || !(ok >> (t8 >> 1) & 1u)) v[k] = 0u;
+                        for (int k = 0; k < 8; ++k) {
+                            const int at = t0 + t8 * 8 + k;
+                            if (at >= w.r.cap || at < w.it.first || !(ok >> (t8 >> 1) & 1u)) v[k] = 0u;
+                        }
                     uint32_t h[4][4];  // [dim][pair of tokens]
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {

@@ -69,10 +69,12 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(Kv8Attn p) {
             for (int f0 = 0; f0 < kTile * CB; f0 += kThreads) {
                 const int f = f0 + tid, row = f / CB, c = f - row * CB, t = t0 + row;
                 int id = -1;
-                if (t < r.cap) id = __ldg(table + (t >> plog));
-                if (id < 0 || id >= p.c.n_pages) {
-                    if (t < r.cap) atomicOr(p.s.err, kKv8ErrRange);
-                    id = -1;
+                if (t < r.cap && t >= (it.first & ~(kKv8Group - 1))) {
+                    id = __ldg(table + (t >> plog));
+                    if (id < 0 || id >= p.c.n_pages) {
+                        atomicOr(p.s.err, kKv8ErrRange);
+                        id = -1;
+                    }
                 }
                 if (c == 0 && (row & (kKv8Group - 1)) == 0) {
                     s_ok[st][row / kKv8Group] = id >= 0;
@@ -85,7 +87,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(Kv8Attn p) {
                     const size_t at = ((((size_t)id * kvh + head) << plog) + (t & (p.c.page_size - 1))) * HD + c * 16;
                     cp_async16(dk, static_cast<const uint8_t*>(p.c.k) + at);
                     cp_async16(dv, static_cast<const uint8_t*>(p.c.v) + at);
-                } else {  // behind the last token: nothing is read
+                } else {  // behind the last token or before the window: nothing is read
                     *reinterpret_cast<uint4*>(dk) = make_uint4(0u, 0u, 0u, 0u);
                     *reinterpret_cast<uint4*>(dv) = make_uint4(0u, 0u, 0u, 0u);
                 }
@@ -145,7 +147,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(Kv8Attn p) {
 #pragma unroll
                 for (int f0 = 0; f0 < kTile * CB; f0 += kThreads) {
                     const int f = f0 + tid, row = f / CB, c = f - row * CB;
-                    const bool zero = t0 + row >= r.cap;
+                    const bool zero = t0 + row >= r.cap || t0 + row < it.first;
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
                         uint4 w = *reinterpret_cast<const uint4*>(rk + kv * kTile * HD + row * HD + c * 16);

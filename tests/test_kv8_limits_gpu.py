@@ -27,6 +27,37 @@ def test_the_largest_windows(iam, cuda, heads, kv, dim, new, dtype, window):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("heads,kv,dim,new,dtype", KERNELS)
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("window,freed", [(37, True), (37, False), (100, True), (100, False)])
+def test_pages_before_the_window(iam, cuda, heads, kv, dim, new, dtype, fmt, window, freed):
+    """A sliding window whose earlier pages have been given back: their table entries name no page, or one that is someone
+    else's by now (codes of NaN, scales of 2^100); tokens before the window in its first page are NaN."""
+    import torch
+    cu, lens, page = offsets(new), [150, 300, 203], 16
+    b = Batch(iam, torch, lens, kv, dim, page, fmt, seed=11)
+    table = b.block_table.clone()
+    stale = next(p for p in range(b.pages) if all(p not in t for t in b.table))
+    for x, s in ((b.k, b.ks), (b.v, b.vs)):
+        x.view(torch.uint8)[stale] = 0x7F
+        s[stale] = 2.0 ** 100
+    q = torch.randn(cu[-1], heads, dim, generator=torch.Generator().manual_seed(6)).to(getattr(torch, dtype)).cuda()
+    want = b.attention_reference(q, cu, window, torch)
+    for i, (n, r) in enumerate(zip(lens, new)):
+        first = max(0, n - r - window + 1)  # the first token that the sequence's first row sees
+        table[i, :first // page] = -1 if freed else stale
+        if first % page:
+            for x in (b.k, b.v):
+                x.view(torch.uint8)[b.table[i][first // page], :, :first % page] = 0x7F
+    cache = iam.KV8Cache(b.k, b.v, b.ks, b.vs, table)
+    out, lse = torch.empty_like(q), torch.empty(cu[-1], heads, device="cuda")
+    h = iam.KV8(heads, kv, dim)
+    h.attention(cache, q, b.seq_lens, out, cu=torch.tensor(cu, dtype=torch.int32, device="cuda"), max_q=max(new), window=window, lse=lse)
+    h.status()
+    close(out, lse, want, torch)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,new,dtype", KERNELS)
 def test_queries_overwritten_by_their_results(iam, cuda, heads, kv, dim, new, dtype):
     """A context long enough that several CTAs share each tile of rows."""
     import torch
