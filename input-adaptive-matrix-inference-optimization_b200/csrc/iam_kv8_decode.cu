@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
             const int t = now.lo + tile * kKv8Group, st = n_used % S::kStages;
             const unsigned char* box_k = mine_ring + st * S::kStage;
             const unsigned char* box_v = box_k + S::kHalves * S::kBox;
-            if (!mbar_wait(&s_full[warp][st], (n_used / S::kStages) & 1, nullptr)) atomicOr(p.s.err, kKv8ErrWait);
+            mbar_wait_unless(&s_full[warp][st], (n_used / S::kStages) & 1, p.s.err, kKv8ErrWait);
             __syncwarp();  // (lanes may leave the wait one by one; the matrix instructions take the warp together)
             const float4 group = s_group[warp][st];
             const float ks_now = group.x, vs_now = group.y;

@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(LogprobParam
     extern __shared__ __align__(16) char s_chunk[];  // [CHUNK] accesses
     __shared__ Part s_part[2][kMaxCluster];          // the cluster's first CTA holds every CTA's part, rows in turn
     __shared__ __align__(8) uint64_t s_full;
+    __shared__ unsigned s_lost;  // 1: a wait gave up, and this row and all later ones are NaN
     __shared__ float s_m[kWarps], s_l[kWarps], s_s[kWarps];
     __shared__ int s_ahead[kWarps];
     __shared__ __align__(16) float s_group[kThreads / 2];
@@ -145,6 +146,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(LogprobParam
     };
     if (C > 1) cluster.barrier_arrive();
     if (tid == 0) {
+        s_lost = 0u;
         mbar_init(&s_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -172,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(LogprobParam
         }
         for (int c0 = w.v0;; c0 += CHUNK) {
             V raw[NV];
-            if (!mbar_wait(&s_full, phase, nullptr)) l = NAN;
+            mbar_wait_unless(&s_full, phase, &s_lost, 1u);
             phase ^= 1u;
             const V* got = reinterpret_cast<const V*>(s_chunk) + tid;
             if (c0 >= w.f0 && c0 + CHUNK <= w.f1) {
@@ -394,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(LogprobParam
             ahead = __reduce_add_sync(0xffffffffu, ahead);
             if (lane == 0) {
                 s_m[warp] = wm;
-                s_l[warp] = l;
+                s_l[warp] = *(volatile unsigned*)&s_lost ? NAN : l;
                 s_s[warp] = s;
                 s_ahead[warp] = ahead;
             }

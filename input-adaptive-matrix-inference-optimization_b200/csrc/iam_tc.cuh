@@ -48,6 +48,21 @@ IAM_DEV bool mbar_wait(uint64_t* b, uint32_t parity, unsigned* err) {
     return true;
 }
 
+// The same for a kernel with many waits: one that lasts (0.5 ms) ends as soon as `word` has one of `bits`, which the first wait to
+// give up sets.  So the kernel's other waits, if they too are for something that never comes, do not each take 2 s.
+IAM_DEV bool mbar_wait_unless(uint64_t* b, uint32_t parity, unsigned* word, unsigned bits) {
+    if (mbar_try_wait(b, parity)) return true;
+    const long long t0 = clock64();
+    while (!mbar_try_wait(b, parity)) {
+        const long long t = clock64() - t0;
+        if (t > kWaitCycles || (t > kWaitCycles / 4096 && (*(volatile unsigned*)word & bits))) {
+            atomicOr(word, bits);
+            return false;
+        }
+    }
+    return true;
+}
+
 // 2-D tiled TMA load of the map's box at (inner c0, row c1); completes bytes on bar.
 IAM_DEV void tma_load_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
     asm volatile(
