@@ -141,3 +141,14 @@ def test_row_tiles_that_end_inside_a_warp(iam, cuda, heads, kv, dim, new, gap):
     close(out, lse, b.attention_reference(q, cu, 0, torch), torch)
     assert (room[cu[-1]:] == 5.0).all() and (room[:, :, :gap] == 5.0).all()
     h.close()
+
+
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("heads,kv,dim,page,fmt,lens,new,window,dtype", [
+    (4, 2, 128, 64, "e4m3", [700], [500], 0, "float32"), (2, 1, 64, 16, "int8", [900, 350], [400, 350], 200, "float32"),
+    (2, 2, 256, 64, "int8", [420], [330], 0, "float32"), (2, 1, 256, 32, "e4m3", [500], [300], 0, "bfloat16"),
+    (4, 1, 256, 128, "int8", [300, 200], [150, 3], 90, "float16")])
+def test_long_prompts_in_fp32_and_of_large_heads(iam, cuda, heads, kv, dim, page, fmt, lens, new, window, dtype):
+    """Several hundred rows in the forms that the tcgen05 kernel does not take."""
+    import torch
+    run(iam, torch, heads, kv, dim, page, fmt, lens, new, window, dtype)

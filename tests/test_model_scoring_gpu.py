@@ -113,3 +113,89 @@ def test_set_rope_refusals(small, iam, cuda):
         with pytest.raises(iam.IamError) as e:
             small.set_rope(iam.Rope.config(**kw))
         assert e.value.code == code
+
+
+@pytest.mark.parametrize("chunk,n", [(7, 30), (1, 5), (16, 33), (29, 30)])
+def test_score_over_several_chunks(iam, cuda, monkeypatch, chunk, n):
+    """Chunks of the prompt one after another in one call, the last one shorter: every output lands at its token.  Bars as for one
+    chunk, against the logits of every prefix."""
+    import torch
+    monkeypatch.setenv("IAM_PREFILL_CHUNK", str(chunk))
+    vocab, k = SMALL["vocab"], 7
+    m = iam.Model.random(iam.ModelConfig.make(**SMALL), seed=7)
+    prompt = np.random.default_rng(n).integers(0, vocab, n).tolist()
+    follow = prompt[1:] + [-1]
+    follow[n // 2] = -1
+    targets = torch.tensor(follow, dtype=torch.int32, device="cuda")
+    out = dict(logprob=torch.full((n,), 99.0, device="cuda"), entropy=torch.full((n,), 99.0, device="cuda"),
+               rank=torch.full((n,), 99, dtype=torch.int32, device="cuda"), top_logprob=torch.full((n, k), 99.0, device="cuda"),
+               top_index=torch.full((n, k), 99, dtype=torch.int32, device="cuda"))
+    nxt = m.score(prompt, targets, **out)
+    logits = torch.empty(vocab, device="cuda")
+    for t in range(n):
+        m.reset()
+        best = m.prefill(prompt[:t + 1], 0, logits)
+        x = logits.double()
+        tol = 2e-3 * float(x.square().mean().sqrt())
+        logp = torch.log_softmax(x, 0)
+        if follow[t] >= 0:
+            assert abs(float(out["logprob"][t]) - float(logp[follow[t]])) < tol
+            mine = float(x[follow[t]])
+            assert int((x > mine + tol).sum()) <= int(out["rank"][t]) <= int((x > mine - tol).sum())
+        else:
+            assert out["logprob"][t] == 0 and out["rank"][t] == -1
+        assert abs(float(out["entropy"][t]) + float((logp.exp() * logp).sum())) < tol * (1 + float(x.abs().max()))
+        assert (out["top_logprob"][t].double() - torch.sort(logp, descending=True)[0][:k]).abs().max() < tol
+        assert (logp[out["top_index"][t].long()] - out["top_logprob"][t].double()).abs().max() < tol
+    assert nxt == best
+    m.close()
+
+
+def test_set_rope_in_decoding(small, iam, cuda):
+    """The ntk scaling is another theta: single steps of the model with it against those of a model made with that theta, and
+    the generation captured before the change against single steps after it.  Between the two models only the angles' last
+    bits differ (as between any two summation orders: logits within 1e-3 x RMS, 5e-2 where a row on a cutoff went the other way)."""
+    import torch
+    m, effort, n, factor = small, 0.5, 24, 2.0
+    d = SMALL["head_dim"]
+    other = iam.Model.random(iam.ModelConfig.make(**SMALL, rope_theta=1e6 * factor ** (d / (d - 2))), seed=7)
+    prompt = np.random.default_rng(4).integers(0, SMALL["vocab"], n).tolist()
+    logits = torch.empty(SMALL["vocab"], device="cuda")
+    gen, again = torch.empty(n, dtype=torch.int32, device="cuda"), torch.empty(n, dtype=torch.int32, device="cuda")
+
+    def steps(model):
+        model.reset()
+        out = []
+        for pos, tok in enumerate(prompt):
+            model.forward(tok, pos, effort, logits)
+            out.append(logits.double().clone())
+        return torch.stack(out)
+
+    def greedy(model):
+        model.reset()
+        tok, out = prompt[0], []
+        for pos in range(n):
+            model.forward(tok, pos, effort, logits)
+            tok = int(logits.argmax())
+            out.append(tok)
+        return out
+
+    plain = steps(m)
+    m.reset()
+    m.generate(prompt[0], 0, n, effort, gen)
+    try:
+        m.set_rope(iam.Rope.config(d, scaling="ntk", factor=factor))
+        scaled = steps(m)
+        m.reset()
+        m.generate(prompt[0], 0, n, effort, again)
+        tokens = greedy(m)
+    finally:
+        m.set_rope(None)
+    want = steps(other)
+    rms = want.square().mean(-1).sqrt()
+    err, change = (scaled - want).abs().amax(-1) / rms, (plain - want).abs().amax(-1) / rms
+    print(f"ntk against theta: median {float(err.median()):.2e}, worst {float(err.max()):.2e}; without it median {float(change.median()):.2e}")
+    assert float(err.max()) < 5e-2 and float(err.median()) < 1e-3 < float(change.median())
+    assert again.tolist() == tokens
+    assert torch.equal(steps(m), plain)
+    other.close()
