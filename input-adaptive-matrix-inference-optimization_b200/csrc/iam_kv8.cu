@@ -367,6 +367,8 @@ extern "C" int iam_kv8_attention(iam_kv8_t h, const iam_kv8_cache* cache, int dt
     const size_t elem = dtype_size(dtype);
     if ((rc = check_rows(q, elem, "queries")) || (rc = check_rows(out, elem, "output"))) return rc;
     if (!seq_lens_dev) return fail(IAM_ERR_ARG, "kv8: null sequence lengths");
+    if (q->data == out->data && ((n_rows > 1 && q->token_stride != out->token_stride) || (h->n_heads > 1 && q->head_stride != out->head_stride)))
+        return fail(IAM_ERR_ARG, "kv8: results over the queries need the same strides for both");
     Kv8Attn a{};
     a.c = *cache;
     a.cu = cu_dev;

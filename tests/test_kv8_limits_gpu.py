@@ -75,6 +75,28 @@ def test_queries_overwritten_by_their_results(iam, cuda, heads, kv, dim, new, dt
 
 
 @pytest.mark.gpu
+def test_results_over_the_queries_at_other_strides_are_refused(iam, cuda):
+    """Row 1's result would lie on queries that are still to be read; one row, or one head, has no such stride."""
+    import torch
+    b = Batch(iam, torch, [40, 40], 2, 64, 16, "int8")
+    h = iam.KV8(4, 2, 64)
+    flat = torch.randn(4 * 4 * 64, device="cuda")
+    q = flat.view(4, 4, 64)[:2]
+    for other in (torch.as_strided(flat, (2, 4, 64), (512, 64, 1)), torch.as_strided(flat, (2, 4, 64), (256, 128, 1)),
+                  torch.as_strided(flat, (2, 4, 64), (64, 128, 1))):
+        with pytest.raises(iam.IamError) as e:
+            h.attention(b.cache, q, b.seq_lens, other)
+        assert e.value.code == iam.IAM_ERR_ARG
+    one = Batch(iam, torch, [40], 2, 64, 16, "int8")
+    apart = torch.empty(1, 4, 64, device="cuda")
+    h.attention(one.cache, q[:1], one.seq_lens, apart)
+    same = torch.as_strided(flat, (1, 4, 64), (777, 64, 1))
+    h.attention(one.cache, q[:1], one.seq_lens, same)
+    h.status()
+    assert torch.equal(same, apart)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("window", [0, 5, 17])
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("heads,kv,dim,dtype", [(4, 2, 64, "float32"), (4, 1, 128, "bfloat16"), (2, 1, 256, "float16"), (24, 1, 64, "float16"),
