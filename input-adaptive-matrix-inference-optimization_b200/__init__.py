@@ -338,6 +338,9 @@ class Rope:
                low_turns=0.0, high_turns=0.0, attn_factor=0.0):
         if scaling not in ROPE_SCALINGS:
             _refuse(f"rope: scaling must be one of {', '.join(ROPE_SCALINGS)}")
+        for what, v in (("head_dim", head_dim), ("rot_dim", rot_dim), ("original_ctx", original_ctx)):
+            if v is not None and not -2 ** 31 <= v < 2 ** 31:
+                _refuse(f"rope: {what} does not fit 32 bits")
         return _RopeConfig(head_dim, head_dim if rot_dim is None else rot_dim, int(bool(interleaved)),
                            ROPE_SCALINGS.index(scaling), theta, factor, original_ctx, low_turns, high_turns, attn_factor)
 
@@ -466,6 +469,8 @@ class KV8:
         """Causal attention of q [rows][n_heads][head_dim] over the sequences' tokens into `out` (q's dtype);
         lse (fp32 [rows][n_heads]) receives the log of the sums.  max_q: a bound on one sequence's rows."""
         self._common(cache, seq_lens, cu, "kv8 attention")
+        if not (0 <= window < 2 ** 31 and 0 <= max_q < 2 ** 31):  # (ctypes would take them modulo 2^32)
+            _refuse("kv8 attention: window and max_q must not be negative and fit 32 bits")
         n, dev = q.shape[0], self.device
         code = _dtype_code(q, "kv8 attention q")
         qr = _rows(q, dev, "kv8 attention q", None, n, self.n_heads, self.head_dim)

@@ -209,3 +209,19 @@ def test_tables_and_rows_beyond_the_limits_are_refused(iam, cuda):
 def test_row_counts_beyond_the_limits_are_refused(iam):
     lib = iam.load_library()
     assert lib.iam_logprobs(None, 0, 2 ** 30 + 1, 8, 8, None, None, None, None, None, 0, None, None, None) == iam.IAM_ERR_ARG
+
+
+@pytest.mark.parametrize("over", [2 ** 31, 2 ** 32, 2 ** 32 + 64, -2 ** 32])
+def test_numbers_beyond_32_bits_are_refused(iam, over):
+    """They would be taken modulo 2^32: a window of 2^32 as none at all.  No handle and no GPU is reached."""
+    h = object.__new__(iam.KV8)
+    h.h, h.device, h.n_heads, h.head_dim = None, 0, 1, 64
+    h._common = lambda *a: None
+    for kw in (dict(window=over), dict(max_q=over)):
+        with pytest.raises(iam.IamError) as e:
+            h.attention(None, None, None, None, **kw)
+        assert e.value.code == iam.IAM_ERR_ARG
+    for kw in (dict(head_dim=over), dict(head_dim=64, rot_dim=over), dict(head_dim=64, original_ctx=over)):
+        with pytest.raises(iam.IamError) as e:
+            iam.Rope.config(**kw)
+        assert e.value.code == iam.IAM_ERR_ARG
