@@ -233,8 +233,8 @@ int iam_rope_apply(iam_rope_t h, int dtype, int n_tokens, const int32_t* positio
 /* A paged cache of keys and values in 8 bits with one fp32 scale per page and KV head, owned by
  * the caller: codes [n_pages][n_kv_heads][page_size][head_dim], scales [n_pages][n_kv_heads], a
  * value being code * scale.  Sequence i keeps token t in page block_table[i * max_pages + t /
- * page_size], row t % page_size.  At most 2^31 rows of codes (n_pages * n_kv_heads * page_size), and
- * 2^26 tokens a sequence.  The scale of a page is the smallest power of two (at least
+ * page_size], row t % page_size.  Fewer than 2^31 rows of codes (n_pages * n_kv_heads * page_size), at
+ * most 2^26 tokens a sequence.  The scale of a page is the smallest power of two (at least
  * 2^-126) that brings every value of the page and head within the largest code (127; 448 for
  * e4m3): dividing by it is exact, so each value is rounded once (to nearest, ties to even), and a
  * page whose scale grows when larger values are appended shifts its older codes. */
@@ -270,9 +270,10 @@ int iam_kv8_append(iam_kv8_t h, const iam_kv8_cache* cache, int dtype, int n_row
  * scale 0: 1/sqrt(head_dim).  out has q's dtype; lse_dev (may be NULL) [n_rows][n_heads] fp32
  * receives the natural logarithm of the sum of exponentials.  A row that sees nothing (a position
  * below 0) gives 0 and -inf.  Scores, maxima and sums are in fp32; the probabilities that multiply the values are
- * rounded to fp16 (11 bits) with 16-bit queries and carry 22 bits with fp32 ones.  out may be q itself (with its strides).  At most 65536 tiles of 64 rows (n_rows * n_heads /
- * n_kv_heads / 64 + n_seqs).  max_q: a bound on one sequence's rows, if known (0: n_rows); it
- * chooses the kernel and never the result's meaning.  What stands in a page behind the sequence's
+ * rounded to fp16 (11 bits) with 16-bit queries and carry 22 bits with fp32 ones.  out may be q itself (with
+ * its strides).  At most 65536 tiles of 64 rows (n_rows * n_heads / n_kv_heads / 64 + n_seqs).  max_q: a bound on
+ * one sequence's rows, if known (0: n_rows; single rows of many sequences under cu_dev want 1, or they are taken
+ * for a prompt); it chooses the kernel and never the result's meaning.  What stands in a page behind the sequence's
  * last token, or before the window of its first row, has no influence, and pages that lie wholly before that window are not
  * looked up (their table entries may name any page or none). */
 int iam_kv8_attention(iam_kv8_t h, const iam_kv8_cache* cache, int dtype, int n_rows, int max_q, const iam_rows* q,

@@ -84,9 +84,9 @@ IAM_DEV int slot_base(int cu, int i, int page_log2) { return (cu >> page_log2) +
 // NT threads (a block, or one warp of it) per (touched page, KV head, K or V), the only ones that write that page and
 // head: pass 1 finds the largest new value, they agree on the scale, pass 2 rounds (and, when the scale grew,
 // shifts the codes that the page held).  Bound by bytes for prompts (the values are read once and kept
-// in registers up to kAppendKeep accesses a thread), by the chain of dependent loads for single tokens.  15000 tokens
-// of 8 heads of 128, bf16 to e4m3 (91 MB): 27.4 us, 3.3 TB/s (half of it the conversions: with the KV heads of a page
-// apart and single conversions 57); 64 sequences of one token: 3.0 us.
+// in registers up to kAppendKeep accesses a thread; of a 64-token page of fp32, half is read twice), by the chain of dependent
+// loads for single tokens.  15000 tokens of 8 heads of 128, bf16 to e4m3 (91 MB): 27.7 us, 3.3 TB/s, with 68 % of the issue slots
+// busy (with the KV heads of a page apart and single conversions 57); fp32 (152 MB): 46 us; 64 sequences of one token: 3.1 us.
 template <class T, int FMT, bool WIDE, int NT>
 __global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(AppendParams p) {
     constexpr int VEC = WIDE ? 16 / (int)sizeof(T) : 4;
@@ -223,7 +223,7 @@ int check_cache(const iam_kv8_cache* c) {
     if (c->n_kv_heads <= 0 || c->n_pages <= 0 || c->max_pages <= 0 || c->n_seqs < 0) return fail(IAM_ERR_ARG, "kv8: bad cache sizes");
     if (c->n_kv_heads > 65535) return fail(IAM_ERR_ARG, "kv8: more than 65535 KV heads");
     if ((long long)c->max_pages * c->page_size > kKv8MaxTokens) return fail(IAM_ERR_UNSUPPORTED, "kv8: a table of more than 2^26 tokens");
-    if ((long long)c->n_pages * c->n_kv_heads * c->page_size > INT32_MAX) return fail(IAM_ERR_UNSUPPORTED, "kv8: more than 2^31 rows of codes");
+    if ((long long)c->n_pages * c->n_kv_heads * c->page_size > INT32_MAX) return fail(IAM_ERR_UNSUPPORTED, "kv8: 2^31 rows of codes or more");
     if (!c->k || !c->v || !c->k_scale || !c->v_scale || (c->n_seqs > 0 && !c->block_table)) return fail(IAM_ERR_ARG, "kv8: null cache array");
     if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16)
         return fail(IAM_ERR_ARG, "kv8: codes must be 16-byte aligned");
@@ -390,11 +390,15 @@ extern "C" int iam_kv8_attention(iam_kv8_t h, const iam_kv8_cache* cache, int dt
     if ((long long)n_rows * a.gq / 64 + cache->n_seqs > kKv8MaxItems)
         return fail(IAM_ERR_ARG, "kv8: more query rows than one call takes (65536 tiles of 64)");
     // The decode kernel reads the context once for 8 rows of a KV head (fp32: 4), the rows kernel once for 64, the prompt
-    // kernel once for 256.  Re-reading from L2 costs less than the others' schedule and join up to 4 passes (head_dim 128,
-    // 32 rows: 1 sequence of 8192 tokens 24 us against 59, 32 of 2000 134 against 150), and up to 8 where the sequences'
-    // KV heads do not fill the SMs by themselves (64 rows: 1 x 8192 38 against 76; but 32 x 2000 252 against 168).  The
-    // prompt kernel takes over where there are many rows (512 of 13 x 2 heads: 184 against 261) or heads to fill the SMs
-    // (128 rows of 32 x 8 heads: 218 against 295; of 4 x 8 heads 108 against 105).
+    // kernel once for 256.  In us, decode | rows | prompt kernel, e4m3, head_dim 128, 8 KV heads where not said: re-reading
+    // from L2 costs less than the others' schedule and join up to 4 passes (32 rows: 1 sequence of 8192 tokens 22 | 60 | 39, 32
+    // of 2000 126 | 151 | 142; fp32, 16 rows: 23 | 63 and 116 | 179), and up to 8 where the sequences' KV heads do not fill
+    // the SMs by themselves (64 rows: 1 x 8192 35 | 76 | 48, but 32 x 2000 234 | 172 | 148; fp32, 32 rows: 36 | 70, but
+    // 218 | 188).  The prompt kernel takes over where there are many rows (512 of 13 x 5000 tokens, 2 KV heads:
+    // 426 | 267 | 130) or heads to fill the SMs (128 of 32 x 2000: 447 | 295 | 166).  Head_dim 64 and 256 lie alike (64 rows of
+    // 1 x 8192: 28 | 50 | 41 and 53 | 118).  The bounds are older than the prompt kernel's present start: between them, where the rows
+    // kernel is still chosen for 16-bit queries, one of the others is faster by now (128 rows of 1 x 8192 58 | 79 | 68, of
+    // 4 x 2000 71 | 78 | 47).
     const long long passes = (rows + (dtype == IAM_F32 ? 3 : 7)) / (dtype == IAM_F32 ? 4 : 8), items = (long long)cache->n_seqs * h->n_kv_heads;
     if (passes <= 4 || (passes <= 8 && items <= h->sms)) return kv8_decode_launch(a, dtype, s);
     if (dtype != IAM_F32 && h->head_dim <= 128 && rows > 64 && (rows > 256 || items >= h->sms)) return kv8_prompt_launch(a, dtype, s);

@@ -1,5 +1,5 @@
 // iam_kv8.h -- the 8-bit paged KV cache: what its launchers take (iam_kv8.cu: handle and append;
-// iam_kv8_decode.cu, iam_kv8_rows.cu: attention of few and of many query rows).
+// iam_kv8_decode.cu, iam_kv8_rows.cu, iam_kv8_prompt.cu: attention of few query rows, of some and of prompts).
 #pragma once
 
 #include <cuda_runtime.h>

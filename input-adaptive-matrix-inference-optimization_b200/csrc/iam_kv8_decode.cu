@@ -6,10 +6,11 @@
 // want of queries.  Which physical dim plays a fragment's k (scores) or row (values) is free as long as the
 // queries and the output agree: the choice below makes every access 16 bytes of adjacent codes of one token.
 //
-// Bound by the codes' bytes in long contexts (one sequence of 131071 tokens, 8 KV heads of 128, 268 MB: 57.1 us, 4.7 TB/s;
-// the conversions to fp16 and the MMAs' issue are next), by the start (finding the run, the first page numbers, scales
-// and copies one after another: 4 us) and the join in short ones (8192 tokens in fp32: 13.4 us for 17 MB).  48 ragged
-// requests (429 MB): 93.4 us, 4.6 TB/s.
+// Long contexts (one sequence of 131071 tokens, 8 KV heads of 128, 268 MB of e4m3: 56.8 us, 4.7 TB/s; int8, whose conversion
+// takes more instructions: 63; 48 ragged requests, 429 MB: 91 us, 4.7 TB/s) are bound by the fixed latencies of a warp's chain from
+// codes to products: the registers allow three warps a scheduler, which issue every second cycle while no unit is more than half
+// busy.  Short ones by the start (finding the run, the first page numbers, scales and copies one after another: 4 us) and
+// the join (8192 tokens in fp32: 13.5 us for 17 MB).
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -21,8 +22,12 @@
 namespace iam {
 namespace {
 
-constexpr int kMinGroups = 8;  // groups of tokens of a CTA at least, where a context is shared
-constexpr int kItemCost = 24;  // what opening and joining a piece of a context costs, in groups
+// Groups of tokens of a CTA at least, where a context is shared (1 x 1024 tokens: 10.5 us; with 4 10.8, with 16 11.6; long
+// contexts do not tell them apart).
+constexpr int kMinGroups = 8;
+// What opening and joining a piece of a context costs, in groups (48 ragged requests 92 us, 200 of up to 600 tokens 59, 13 x 7 drafted
+// rows 34; with 8 groups 101, 70, 63; with 48 98, 64, 31; with 96 109, 67, 36).
+constexpr int kItemCost = 24;
 // Probabilities (at most 1) are lifted by this before they are rounded to fp16, whose smallest step is 2^-24: a weight of 2^-28
 // still has all of its 11 bits, and what is lost of smaller ones is 2^-39 of the largest value a token.
 constexpr float kLift = 16384.0f;

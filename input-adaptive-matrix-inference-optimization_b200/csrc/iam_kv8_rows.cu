@@ -17,7 +17,8 @@ constexpr int kMinUnits = 8;    // units of a CTA at least, while there are enou
 // probabilities (fp16, one or two terms) from the accumulators' own registers as A and the values as B.
 // Codes arrive by cp.async one tile ahead and become fp16 in shared memory once per tile for all warps.  Bound by the
 // MMAs' and the softmax's issue.  This kernel serves what the other two do not: 64 rows of one 8192-token
-// sequence take it 76 us (the decode kernel 38), of 32 x 2000 tokens 168 (252); fp32 and head_dim 256 prompts always.
+// sequence take it 76 us (the decode kernel 35), of 32 x 2000 tokens 172 (234); fp32 and head_dim 256 prompts always (2048 rows on
+// 8192 earlier tokens: 32 heads of 128 over 8 in fp32 2716 us, 8 heads of 256 over 1 in bf16 1524, in fp32 1895).
 template <class T, int FMT, int HD, int TERMS>
 __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(Kv8Attn p) {
     constexpr int KS = HD / 16, NT = kTile / 8, CB = HD / 16;  // CB: 16-byte pieces of a code row

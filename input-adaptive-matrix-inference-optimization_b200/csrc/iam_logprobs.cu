@@ -98,8 +98,10 @@ IAM_DEV float before(float x) {
 // The alternatives: of the maxima of 64 groups of threads (128 when more than 32 are wanted) the k-th largest is a
 // lower bound of the chunk's, and so of the row's, k-th largest value, and hardly more than k values reach it; these
 // are collected and ranked.
-// 2048 rows of 32000 (fp32, 262 MB): 49 us without alternatives (5.3 TB/s), 116 with 20: the threads' comparisons among
-// groups, the collection and the ranking are a chain of barriers that two CTAs an SM hide only in part.  One row: 7.1 us.
+// 2048 rows of 32000 (262 MB in fp32): 50 us without alternatives (5.2 TB/s; bf16 48), 95 with 20 (127): the threads'
+// comparisons among groups, the collection and the ranking are a chain of barriers that two CTAs an SM hide only in part.  With
+// -inf in a tenth of every third row's tokens 79 and 117 (55 and 133): a target among them is counted element by element, and its
+// row holds up its CTA.  One row: 7.7 us.
 template <class T, int NV>
 __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(LogprobParams p, int n_rows) {
     constexpr int VEC = 16 / (int)sizeof(T), CHUNK = NV * kThreads;

@@ -78,7 +78,8 @@ struct RopeParams {
 // walks the (token, head) rows, which are spread over the block and blockIdx.y.  Bound by the bytes; the angles cost one
 // reduction in 64 bits and one sincospif per pair and token, shared by all its heads through shared memory.  2048
 // tokens of 32 + 8 heads of 128 (bf16, 42 MB): 11.1 us, 3.8 TB/s; 8191 tokens of 16 + 16 heads, 64 of 128 dims
-// interleaved (fp16, 134 MB): 35.2 us, 3.8 TB/s; one token: 2.1 us, the launch.  (Rows asked for before the angles are
+// interleaved (fp16, 134 MB): 35.2 us, 3.8 TB/s (in place 36.6: the dims that do not turn are moved all the same); one token: 2.1 us,
+// the launch.  (Rows asked for before the angles are
 // made, one to four a thread, took 12.4 to 20 us for the first.)  The angle in turns is exact to 2^-53 of its size, so a position of 2^31 still has its phase to 2^-24.
 template <class T, bool INTER, bool WIDE>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeParams p, int group) {
