@@ -13,9 +13,9 @@
 //   13           the copies (TMA, 16 rows a box, so any page size)
 // 128 x 128 rows and tokens cost the tensor cores 512 cycles for S and as many for P V (head_dim 128), and their 16384
 // powers cost the special-function units 1024: the two are level, and neither can wait for the other.  2048 rows on 8192
-// earlier tokens (32 heads of 128 over 8): 497 us, 623 TFLOP/s
-// (queries and results moved 2 bytes at a time: 606); 2 x 141 rows on 222 tokens 85, nearly all of it start and join.  Bound by the softmax's chain from one tile's scores to
-// its probabilities, some 3200 cycles for 256 x 64; the mma.sync kernel for rows took 2001.
+// earlier tokens (32 heads of 128 over 8): 497 us, 623 TFLOP/s (queries and results moved 2 bytes at a time: 606); 2 x 141 rows
+// on 222 tokens 85, nearly all of it start and join.  Bound by the softmax's chain from one tile's scores to its
+// probabilities, some 3200 cycles for 256 x 64; the mma.sync kernel for rows took 2001.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
