@@ -275,7 +275,8 @@ int iam_kv8_append(iam_kv8_t h, const iam_kv8_cache* cache, int dtype, int n_row
  * one sequence's rows, if known (0: n_rows; single rows of many sequences under cu_dev want 1, or they are taken
  * for a prompt); it chooses the kernel and never the result's meaning.  What stands in a page behind the sequence's
  * last token, or before the window of its first row, has no influence, and pages that lie wholly before that window are not
- * looked up (their table entries may name any page or none). */
+ * looked up (their table entries may name any page or none).  A NaN among the codes or scales in between (the append writes
+ * none) may reach every row of its sequence, those before it too. */
 int iam_kv8_attention(iam_kv8_t h, const iam_kv8_cache* cache, int dtype, int n_rows, int max_q, const iam_rows* q,
                       const int32_t* cu_dev, const int32_t* seq_lens_dev, float scale, int window, const iam_rows* out,
                       float* lse_dev, void* stream);
